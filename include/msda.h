@@ -330,6 +330,116 @@ int msda_point_sample_backward(const void* grad_out, const void* input, const vo
  */
 size_t msda_point_sample_workspace_bytes(int N, int C, int H, int W, int P, int dtype);
 
+/* ---------------------------------------------------------------------------------------------
+ * Operators around the attention of an encoder layer: dropout, residual + layer norm, group norm
+ * of the pyramid.  No counterpart in the reference (its modules call torch's own operators).
+ *
+ * Element types: F32, F64, BF16, F16.  16-bit types compute in fp32; every sum, mean and variance
+ * is held in fp32 (fp64 for F64) and added in an order that the sizes alone fix, so results are
+ * reproducible bit for bit.  "Compute type" below: F64 for F64, F32 for the others.
+ * Pointers need the alignment of their element type only, and rows may have any width.
+ * No entry point writes any memory but its outputs and its workspace.
+ * --------------------------------------------------------------------------------------------- */
+
+/* activations */
+enum {
+  MSDA_ACT_NONE = 0,
+  MSDA_ACT_RELU = 1,
+  MSDA_ACT_SILU = 2, /* z * sigmoid(z) */
+  MSDA_ACT_GELU = 3, /* z * Phi(z), Phi the normal distribution function (no tanh form) */
+};
+
+/*
+ * Dropout whose mask is computed from counters and never stored:
+ *     out[i] = keep(i) ? act(x[i]) / (1 - p) : 0,       act = identity or MSDA_ACT_RELU
+ * keep(i) is a function of (rng_state, site, i) alone: 16 bits u(i) of Philox4x32 with 7 rounds
+ * (Salmon, Moraes, Dror, Shaw 2011), counter (i / 8, site, offset low, offset high), key
+ * (seed low, seed high), element i taking the low (even i) or high half of word (i % 8) / 2;
+ * keep(i) = u(i) >= t with t = round(65536 p), and 1 / (1 - p) stands for 65536 / (65536 - t)
+ * (0 < p < 1 is kept within 1 .. 65535 of 65536; p = 0 drops nothing, p = 1 everything).
+ *
+ * `rng_state`: two int64 in DEVICE memory, (seed, offset), read when the kernel runs: a captured
+ * graph draws new masks on every replay if the caller changes them in between.  `site` >= 0 tells
+ * the uses of one state apart.  `rng_state` may be NULL when p = 0.  A dropped element is 0
+ * whatever x holds (NaN and infinities included); a kept NaN stays.  `out` may be `x`.
+ * numel <= 2^35 when p > 0 (MSDA_ESHAPE).
+ */
+int msda_dropout_forward(const void* x, void* out, const int64_t* rng_state, int64_t numel,
+                         double p, int site, int activation, int dtype, void* hip_stream);
+
+/*
+ * grad_x of msda_dropout_forward.  MSDA_ACT_NONE: grad_x = keep ? grad_out / (1 - p) : 0, from the
+ * same (rng_state, site); `out` is ignored.  MSDA_ACT_RELU: from the forward's output `out`
+ * (grad_x = out <= 0 ? 0 : grad_out / (1 - p)); `rng_state` and `site` are ignored.
+ * `grad_x` may be `grad_out`.
+ */
+int msda_dropout_backward(const void* grad_out, const void* out, void* grad_x,
+                          const int64_t* rng_state, int64_t numel, double p, int site,
+                          int activation, int dtype, void* hip_stream);
+
+/*
+ * out = LayerNorm(residual + dropout(x)) * weight + bias over the C columns of each of `rows` rows
+ * (biased variance, eps inside the root); the mask of element (r, c) is that of
+ * msda_dropout_forward at index r * C + c.  `residual` and `out` have dtype_residual: dtype_x, or
+ * F32 next to a 16-bit x; `weight` and `bias` (C) have dtype_residual, or F32 next to 16 bits.
+ * `mean`, `rstd` (rows, compute type of dtype_residual) receive what the backward needs; both may
+ * be NULL.  Rows of up to 16384 bytes of dtype_residual (MSDA_ESHAPE).
+ */
+int msda_dropout_add_norm_forward(const void* x, const void* residual, const void* weight,
+                                  const void* bias, void* out, void* mean, void* rstd,
+                                  const int64_t* rng_state, int64_t rows, int C, double p, int site,
+                                  double eps, int dtype_x, int dtype_residual, int dtype_param,
+                                  void* hip_stream);
+
+/* Scratch of msda_dropout_add_norm_backward in bytes (8-byte aligned); 0 for invalid arguments. */
+size_t msda_dropout_add_norm_workspace_bytes(int64_t rows, int C, int dtype_x, int dtype_residual);
+
+/*
+ * Gradients of msda_dropout_add_norm_forward.  grad_x (dtype_x) and grad_residual
+ * (dtype_residual) may each be NULL where not wanted (with p = 0 and equal types they are equal);
+ * grad_weight and grad_bias (dtype_param) may be NULL together, and `workspace` with them.
+ */
+int msda_dropout_add_norm_backward(const void* grad_out, const void* x, const void* residual,
+                                   const void* weight, const void* mean, const void* rstd,
+                                   void* grad_x, void* grad_residual, void* grad_weight,
+                                   void* grad_bias, void* workspace, size_t workspace_bytes,
+                                   const int64_t* rng_state, int64_t rows, int C, double p,
+                                   int site, int dtype_x, int dtype_residual, int dtype_param,
+                                   void* hip_stream);
+
+/*
+ * Group normalisation of a flattened pyramid, channels last, with an activation:
+ * x (N, S, C); level l covers level_rows_host[l] consecutive rows of every sample (HOST memory,
+ * read during the call; they add up to S).  Each (sample, level, group of C / G channels) is
+ * normalised on its own (biased variance, eps inside the root):
+ *     out = act((x - mean) * rstd * weight + bias)
+ * `weight`, `bias` (param_levels, C), param_levels = L (one set a level) or 1, of `dtype`, or F32
+ * next to 16 bits.  `mean`, `rstd` (N, L, G), compute type, receive what the backward needs; both
+ * may be NULL.  L <= 16 (MSDA_ELEVELS); rows of up to 16384 bytes (MSDA_ESHAPE).
+ * `workspace`: msda_group_norm_workspace_bytes(...) bytes with backward = 0, 8-byte aligned.
+ */
+int msda_group_norm_forward(const void* x, const void* weight, const void* bias, void* out,
+                            void* mean, void* rstd, void* workspace, size_t workspace_bytes,
+                            const int64_t* level_rows_host, int N, int S, int C, int G, int L,
+                            int param_levels, double eps, int activation, int dtype,
+                            int dtype_param, void* hip_stream);
+
+/* Scratch of the group norm's forward (backward = 0) or backward (1); 0 for invalid arguments. */
+size_t msda_group_norm_workspace_bytes(const int64_t* level_rows_host, int N, int S, int C, int G,
+                                       int L, int dtype, int backward);
+
+/*
+ * Gradients of msda_group_norm_forward from its inputs and its mean and rstd.  grad_x may be NULL
+ * where not wanted; grad_weight and grad_bias (shape and type of weight) may be NULL together.
+ * The gradient of MSDA_ACT_RELU at 0 is 0.
+ */
+int msda_group_norm_backward(const void* grad_out, const void* x, const void* weight,
+                             const void* bias, const void* mean, const void* rstd, void* grad_x,
+                             void* grad_weight, void* grad_bias, void* workspace,
+                             size_t workspace_bytes, const int64_t* level_rows_host, int N, int S,
+                             int C, int G, int L, int param_levels, int activation, int dtype,
+                             int dtype_param, void* hip_stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,351 @@
+"""The operators around the attention where no GPU is needed: the oracle's generator against its
+published vectors, the oracle's gradients against differences, argument checks of the Python surface
+and of the C ABI (nothing is launched), shapes under torch's fake tensors."""
+
+from __future__ import annotations
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import epilogue_ref as ref
+from unipercept_amd import _lib
+from unipercept_amd.deform_attn import (
+    LevelInputProjection,
+    MSDeformAttnEncoder,
+    MSDeformAttnEncoderLayer,
+    counter_dropout,
+    dropout_add_layer_norm,
+    flatten_levels,
+    level_group_norm,
+    new_rng_state,
+)
+from unipercept_amd.deform_attn import _epilogue_ops as ops
+
+FAKE = 0x1000  # never dereferenced: every call below fails validation first
+
+
+# ---- the oracle itself ----------------------------------------------------------------------------
+
+
+def test_generator_known_answers():
+    """Vectors published with the generator (zeros; 10 rounds also with all bits set)."""
+    z, f = 0, 0xFFFFFFFF
+    assert [int(v) for v in ref.philox4x32((z,) * 4, (z,) * 2, 7)] == [
+        0x5F6FB709, 0x0D893F64, 0x4F121F81, 0x4F730A48]
+    assert [int(v) for v in ref.philox4x32((z,) * 4, (z,) * 2, 10)] == [
+        0x6627E8D5, 0xE169C58D, 0xBC57AC4C, 0x9B00DBD8]
+    assert [int(v) for v in ref.philox4x32((f,) * 4, (f,) * 2, 10)] == [
+        0x408F276D, 0x41C83B0E, 0xA20BC7C6, 0x6D5451FD]
+
+
+def test_keep_bits_statistics_and_windows():
+    n, p = 1 << 16, 0.1
+    k = ref.keep(0, n, p, -5, 3, 2)
+    # 5 standard deviations of a binomial count
+    assert abs(k.sum() - n * (1 - round(p * 65536) / 65536)) < 5 * (n * p * (1 - p)) ** 0.5
+    assert np.array_equal(ref.keep(1003, 77, p, -5, 3, 2), k[1003:1080])
+    for other in (ref.keep(0, n, p, -5, 3, 1), ref.keep(0, n, p, -5, 4, 2), ref.keep(0, n, p, -6, 3, 2)):
+        agree = (other == k).mean()
+        assert abs(agree - (p * p + (1 - p) ** 2)) < 0.01  # as independent masks do
+
+
+@pytest.mark.parametrize("p,t", [(0.0, 0), (1e-9, 1), (0.1, 6554), (0.5, 32768), (1 - 1e-9, 65535), (1.0, 65536)])
+def test_probability_steps(p, t):
+    assert ref.threshold(p) == t
+
+
+def _difference(f, x, d):
+    h = 1e-6
+    return ((f(x + h * d) - f(x - h * d)) / (2 * h)).item()
+
+
+@pytest.mark.parametrize("activation", ["none", "relu", "silu", "gelu"])
+def test_oracle_gradients_against_differences(activation):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 7, 6, generator=g, dtype=torch.float64)
+    dy = torch.randn(2, 7, 6, generator=g, dtype=torch.float64)
+    w = torch.randn(2, 6, generator=g, dtype=torch.float64)
+    b = torch.randn(2, 6, generator=g, dtype=torch.float64)
+    rows = [4, 3]
+
+    def value(x, w, b):
+        return (ref.group_norm(x, w, b, 3, rows, 1e-5, activation)[0] * dy).sum()
+
+    grads = ref.group_norm_grad(dy, ref.group_norm(x, w, b, 3, rows, 1e-5, activation)[1], activation)
+    for k, t in enumerate((x, w, b)):
+        d = torch.randn(t.shape, generator=g, dtype=torch.float64)
+        got = _difference(lambda v: value(*[v if i == k else a for i, a in enumerate((x, w, b))]), t, d)
+        assert abs(got - (grads[k] * d).sum().item()) < 1e-6 * (1 + abs(got))
+    if activation in ("silu", "gelu"):
+        return
+    state = (123456789, -7)
+    got = _difference(lambda v: (ref.dropout(v, 0.3, state, 4, activation) * dy).sum(), x, dy)
+    assert abs(got - (ref.dropout_grad(dy, x, 0.3, state, 4, activation) * dy).sum().item()) < 1e-6 * (1 + abs(got))
+    if activation == "none":
+        args = [x, x.flip(0).contiguous(), w[0], b[0]]
+
+        def norm(args):
+            return (ref.add_norm(*args, 0.3, state, 1, 1e-5)[0] * dy).sum()
+
+        grads = ref.add_norm_grad(dy, w[0], ref.add_norm(*args, 0.3, state, 1, 1e-5)[1])
+        for k, t in enumerate(args):
+            d = torch.randn(t.shape, generator=g, dtype=torch.float64)
+            got = _difference(lambda v: norm([v if i == k else a for i, a in enumerate(args)]), t, d)
+            assert abs(got - (grads[k] * d).sum().item()) < 1e-6 * (1 + abs(got))
+
+
+# ---- refusals of the Python surface -----------------------------------------------------------------
+
+
+def meta(*shape, dtype=torch.float32):
+    return torch.empty(shape, dtype=dtype, device="meta")
+
+
+STATE = torch.empty(2, dtype=torch.int64, device="meta")
+
+
+@pytest.mark.parametrize(
+    "args,kw,exc",
+    [
+        ((torch.zeros(4), 0.1, torch.zeros(2, dtype=torch.int64)), {}, RuntimeError),  # CPU tensor
+        ((meta(4, dtype=torch.int32), 0.1, STATE), {}, TypeError),
+        ((meta(4), -0.1, STATE), {}, ValueError),
+        ((meta(4), 1.1, STATE), {}, ValueError),
+        ((meta(4), float("nan"), STATE), {}, ValueError),
+        ((meta(4), 0.1), {}, ValueError),  # no state
+        ((meta(4), 0.1, meta(3, dtype=torch.int64)), {}, ValueError),
+        ((meta(4), 0.1, meta(2)), {}, ValueError),
+        ((meta(4), 0.1, torch.zeros(2, dtype=torch.int64)), {}, RuntimeError),  # another device
+        ((meta(4), 0.1, STATE), {"site": -1}, ValueError),
+        ((meta(4), 0.1, STATE), {"site": 2**31}, ValueError),
+        ((meta(4), 0.1, STATE), {"activation": "silu"}, ValueError),
+        ((meta(2**18, 2**18, dtype=torch.bfloat16), 0.1, STATE), {}, ValueError),  # 2^36 elements
+    ],
+)
+def test_dropout_refusals(args, kw, exc):
+    with pytest.raises(exc):
+        counter_dropout(*args, **kw)
+
+
+def test_dropout_of_nothing_is_the_input():
+    x = meta(4)
+    assert counter_dropout(x, 0.0) is x
+
+
+NORM = dict(x=meta(3, 8), residual=meta(3, 8), weight=meta(8), bias=meta(8))
+BF = torch.bfloat16
+
+
+@pytest.mark.parametrize(
+    "change,exc",
+    [
+        (dict(x=torch.zeros(3, 8)), RuntimeError),
+        (dict(residual=meta(3, 9)), ValueError),
+        (dict(residual=meta(3, 8, dtype=BF)), TypeError),  # a residual narrower than x
+        (dict(x=meta(3, 8, dtype=torch.float64)), TypeError),
+        (dict(x=meta(3, 8, dtype=BF), residual=meta(3, 8, dtype=torch.float16)), TypeError),
+        (dict(weight=meta(9), bias=meta(9)), ValueError),
+        (dict(weight=meta(8, dtype=BF)), ValueError),  # weight and bias differ
+        (dict(weight=meta(8, dtype=BF), bias=meta(8, dtype=BF)), TypeError),  # narrower than x
+        (dict(weight=torch.zeros(8), bias=torch.zeros(8)), RuntimeError),
+        (dict(eps=-1e-5), ValueError),
+        (dict(eps=float("nan")), ValueError),
+        (dict(p=0.1), ValueError),
+        (dict(p=2.0, rng_state=STATE), ValueError),
+        (dict(x=meta(2, 4100), residual=meta(2, 4100), weight=meta(4100), bias=meta(4100)), ValueError),
+        (dict(x=meta(3, 0), residual=meta(3, 0), weight=meta(0), bias=meta(0)), ValueError),
+        (dict(x=meta(), residual=meta()), ValueError),
+    ],
+)
+def test_add_norm_refusals(change, exc):
+    with pytest.raises(exc):
+        dropout_add_layer_norm(**{**NORM, **change})
+
+
+GROUP = dict(x=meta(2, 20, 8), weight=meta(8), bias=meta(8), num_groups=4)
+
+
+@pytest.mark.parametrize(
+    "change,exc",
+    [
+        (dict(x=torch.zeros(2, 20, 8)), RuntimeError),
+        (dict(x=meta(8)), ValueError),
+        (dict(num_groups=3), ValueError),
+        (dict(num_groups=0), ValueError),
+        (dict(spatial_shapes=[(4, 4)]), ValueError),  # 16 of 20 positions
+        (dict(spatial_shapes=[(4, 4), (0, 9), (2, 2)]), ValueError),
+        (dict(spatial_shapes=[(1, 1)] * 20), ValueError),  # more than 16 levels
+        (dict(x=meta(2, 4, 5, 8), spatial_shapes=[(4, 5)]), ValueError),
+        (dict(weight=meta(3, 8), bias=meta(3, 8), spatial_shapes=[(4, 4), (2, 2)]), ValueError),
+        (dict(weight=meta(8, dtype=BF), bias=meta(8, dtype=BF)), TypeError),
+        (dict(bias=meta(2, 8)), ValueError),
+        (dict(activation="tanh"), ValueError),
+        (dict(eps=-1.0), ValueError),
+        (dict(x=meta(1, 2, 8200, dtype=BF), weight=meta(8200), bias=meta(8200)), ValueError),
+        (dict(x=meta(2, 20, 8, dtype=torch.int64)), TypeError),
+    ],
+)
+def test_group_norm_refusals(change, exc):
+    with pytest.raises(exc):
+        level_group_norm(**{**GROUP, **change})
+
+
+def test_shapes_and_types_without_running():
+    x = meta(2, 20, 8, dtype=BF)
+    shapes = [(4, 4), (2, 2)]
+    assert counter_dropout(x, 0.1, STATE).shape == x.shape
+    y = level_group_norm(x, meta(2, 8), meta(2, 8), 4, shapes)
+    assert y.shape == x.shape and y.dtype == BF
+    z = dropout_add_layer_norm(x, meta(2, 20, 8), meta(8), meta(8))
+    assert z.shape == x.shape and z.dtype == torch.float32
+    out, mean, rstd = torch.ops.unipercept.level_group_norm_fwd(x, meta(8), meta(8), 4, [16, 4], 1e-5, "none", True)
+    assert mean.shape == rstd.shape == (2, 2, 4) and mean.dtype == torch.float32
+    gx, gr, gw, gb = torch.ops.unipercept.dropout_add_norm_bwd(
+        z, x, z, meta(8), meta(40), meta(40), None, 0.0, 0, True, False, True)
+    assert gx.dtype == BF and gr.numel() == 0 and gw.shape == gb.shape == (8,)
+    assert new_rng_state("cpu").shape == (2,) and new_rng_state("cpu").dtype == torch.int64
+
+
+def test_level_rows_come_from_lists_tensors_and_plain_shapes():
+    x = meta(2, 20, 8)
+    assert ops.level_rows(x, [(4, 4), (2, 2)]) == [16, 4]
+    assert ops.level_rows(x, torch.tensor([[4, 4], [2, 2]])) == [16, 4]
+    assert ops.level_rows(meta(2, 4, 5, 8), None) == [20]
+    assert ops.level_rows(meta(2, 8), None) == [1]
+
+
+# ---- argument errors of the C ABI -------------------------------------------------------------------
+
+
+def test_abi_dropout_errors():
+    lib = _lib.load()
+
+    def fwd(x=FAKE, out=FAKE, state=FAKE, numel=8, p=0.1, site=0, act=0, dtype=0):
+        return lib.msda_dropout_forward(x, out, state, numel, p, site, act, dtype, None)
+
+    def bwd(g=FAKE, out=FAKE, gx=FAKE, state=FAKE, numel=8, p=0.1, site=0, act=1, dtype=0):
+        return lib.msda_dropout_backward(g, out, gx, state, numel, p, site, act, dtype, None)
+
+    assert fwd(x=None) == -1 and fwd(out=None) == -1 and fwd(state=None) == -1
+    assert bwd(g=None) == -1 and bwd(gx=None) == -1 and bwd(out=None) == -1
+    assert bwd(act=0, state=None) == -1
+    assert fwd(numel=0) == -2 and fwd(p=-0.1) == -2 and fwd(p=1.5) == -2 and fwd(p=float("nan")) == -2
+    assert fwd(site=-1) == -2 and fwd(numel=(1 << 35) + 1) == -2
+    assert fwd(dtype=9) == -3 and fwd(act=2) == -3 and bwd(act=3) == -3 and bwd(dtype=-1) == -3
+    assert fwd(x=FAKE + 2) == -4 and fwd(state=FAKE + 4) == -4 and bwd(gx=FAKE + 1, dtype=2) == -4
+
+
+def test_abi_add_norm_errors():
+    lib = _lib.load()
+    need = lib.msda_dropout_add_norm_workspace_bytes
+
+    def fwd(x=FAKE, res=FAKE, w=FAKE, b=FAKE, out=FAKE, mean=FAKE, rstd=FAKE, state=FAKE, rows=4, c=8,
+            p=0.1, site=0, eps=1e-5, dx=0, dr=0, dp=0):
+        return lib.msda_dropout_add_norm_forward(
+            x, res, w, b, out, mean, rstd, state, rows, c, p, site, eps, dx, dr, dp, None)
+
+    def bwd(g=FAKE, x=FAKE, res=FAKE, w=FAKE, mean=FAKE, rstd=FAKE, gx=FAKE, gr=FAKE, gw=FAKE, gb=FAKE,
+            ws=FAKE, nbytes=1 << 20, state=FAKE, rows=4, c=8, p=0.1, site=0, dx=0, dr=0, dp=0):
+        return lib.msda_dropout_add_norm_backward(
+            g, x, res, w, mean, rstd, gx, gr, gw, gb, ws, nbytes, state, rows, c, p, site, dx, dr, dp, None)
+
+    for name in ("x", "res", "w", "b", "out", "state"):
+        assert fwd(**{name: None}) == -1
+    assert fwd(mean=None) == -1 and fwd(rstd=None) == -1  # both or neither
+    for name in ("g", "x", "res", "w", "mean", "rstd", "state"):
+        assert bwd(**{name: None}) == -1
+    assert bwd(gw=None) == -1 and bwd(gb=None) == -1
+    for call in (fwd, bwd):
+        assert call(rows=0) == -2 and call(c=0) == -2 and call(rows=1 << 31) == -2 and call(c=4097) == -2
+        assert call(p=1.01) == -2 and call(site=-3) == -2
+        assert call(dx=9) == -3 and call(dx=0, dr=2) == -3 and call(dx=2, dr=3, dp=3) == -3
+        assert call(dx=2, dr=0, dp=2) == -3 and call(dx=1, dr=1, dp=0) == -3
+        assert call(x=FAKE + 2) == -4 and call(rstd=FAKE + 2) == -4 and call(state=FAKE + 4) == -4
+        assert call(dx=1, dr=1, dp=1, c=2049) == -2  # 16 KiB of the residual's type
+    assert fwd(eps=-1.0) == -2 and fwd(eps=float("nan")) == -2
+    assert bwd(ws=None) == -5 and bwd(ws=FAKE + 4) == -5 and bwd(nbytes=need(4, 8, 0, 0) - 1) == -5
+    # sums of two per column and workgroup; at most 1024 workgroups
+    assert need(4, 8, 0, 0) == 4 * 2 * 8 * 4 and need(10**6, 256, 2, 0) == 1024 * 2 * 256 * 4
+    assert need(4, 8, 1, 1) == 4 * 2 * 8 * 8 and need(0, 8, 0, 0) == 0 and need(4, 8, 0, 2) == 0
+
+
+def test_abi_group_norm_errors():
+    lib = _lib.load()
+    need = lib.msda_group_norm_workspace_bytes
+
+    def host(rows):
+        return (ctypes.c_int64 * len(rows))(*rows)
+
+    def fwd(x=FAKE, w=FAKE, b=FAKE, out=FAKE, mean=FAKE, rstd=FAKE, ws=FAKE, nbytes=1 << 24, rows=(16, 4),
+            n=2, s=20, c=8, g=4, l=2, pl=1, eps=1e-5, act=0, dtype=0, dp=0):
+        return lib.msda_group_norm_forward(
+            x, w, b, out, mean, rstd, ws, nbytes, rows and host(rows), n, s, c, g, l, pl, eps, act, dtype, dp, None)
+
+    def bwd(gy=FAKE, x=FAKE, w=FAKE, b=FAKE, mean=FAKE, rstd=FAKE, gx=FAKE, gw=FAKE, gb=FAKE, ws=FAKE,
+            nbytes=1 << 24, rows=(16, 4), n=2, s=20, c=8, g=4, l=2, pl=1, act=0, dtype=0, dp=0):
+        return lib.msda_group_norm_backward(
+            gy, x, w, b, mean, rstd, gx, gw, gb, ws, nbytes, rows and host(rows), n, s, c, g, l, pl, act,
+            dtype, dp, None)
+
+    for name in ("x", "w", "b", "out", "mean", "rstd", "rows"):
+        assert fwd(**{name: None}) == -1
+    for name in ("gy", "x", "w", "b", "mean", "rstd", "gw", "gb", "rows"):
+        assert bwd(**{name: None}) == -1
+    for call in (fwd, bwd):
+        assert call(n=0) == -2 and call(s=0) == -2 and call(c=0) == -2 and call(g=0) == -2 and call(l=0) == -2
+        assert call(g=3) == -2 and call(pl=3) == -2 and call(pl=0) == -2
+        assert call(rows=(16, 5)) == -2 and call(rows=(21, -1)) == -2 and call(rows=(20, 0)) == -2
+        assert call(rows=(1,) * 17, l=17, s=17) == -7
+        assert call(c=4100) == -2 and call(n=1 << 30) == -2
+        assert call(dtype=9) == -3 and call(act=4) == -3 and call(act=-1) == -3 and call(dp=2) == -3
+        assert call(dtype=1, dp=0) == -3 and call(dtype=2, dp=3) == -3
+        assert call(x=FAKE + 2) == -4 and call(mean=FAKE + 2) == -4
+        assert call(ws=None) == -5 and call(ws=FAKE + 4) == -5 and call(nbytes=0) == -5
+    assert fwd(eps=float("nan")) == -2
+    rows = host((16, 4))
+    assert need(rows, 2, 20, 8, 4, 2, 0, 0) > 0 and need(rows, 2, 20, 8, 4, 2, 0, 1) > need(rows, 2, 20, 8, 4, 2, 0, 0)
+    assert need(rows, 2, 21, 8, 4, 2, 0, 0) == 0 and need(None, 2, 20, 8, 4, 2, 0, 0) == 0
+
+
+# ---- the modules --------------------------------------------------------------------------------------
+
+
+def test_encoder_layers_keep_their_parameters_and_default_route():
+    plain = MSDeformAttnEncoderLayer(32, 48, 0.1, n_levels=2, n_heads=4, n_points=2)
+    fused = MSDeformAttnEncoderLayer(32, 48, 0.1, n_levels=2, n_heads=4, n_points=2, fused_epilogues=True)
+    assert not plain.fused_epilogues
+    fused.load_state_dict(plain.state_dict())
+    enc = MSDeformAttnEncoder(2, d_model=32, d_ffn=48, n_levels=2, n_heads=4, n_points=2, fused_epilogues=True)
+    assert all(layer.fused_epilogues for layer in enc.layers)
+
+
+def test_encoder_passes_its_old_arguments_to_foreign_layers():
+    """Layers put in place of the stack's own are called with the arguments they always were."""
+
+    class Foreign(torch.nn.Module):
+        def forward(self, src, pos, ref, shapes, lsi, mask):
+            return src + 1
+
+    enc = MSDeformAttnEncoder(1, d_model=16, d_ffn=32, n_levels=1, n_heads=2, n_points=2)
+    enc.layers[0] = Foreign()
+    src, shapes, lsi, levels, _ = flatten_levels([torch.zeros(1, 16, 2, 3)])
+    assert torch.equal(enc(src, shapes, lsi, spatial_shapes_list=levels), src + 1)
+
+
+def test_fused_routes_refuse_cpu_tensors():
+    src, shapes, lsi, levels, _ = flatten_levels([torch.zeros(1, 16, 2, 3)])
+    layer = MSDeformAttnEncoderLayer(16, 32, 0.0, n_levels=1, n_heads=2, n_points=2, fused_epilogues=True)
+    with pytest.raises(RuntimeError, match="only on a ROCm GPU"):
+        layer._fused_rest(src, src, None, 0)
+    with pytest.raises(RuntimeError, match="only on a ROCm GPU"):
+        LevelInputProjection([16], 16, 4)([torch.zeros(1, 16, 2, 3)])
+
+
+def test_input_projection_checks():
+    with pytest.raises(ValueError, match="divisible"):
+        LevelInputProjection([16], 20, 8)
+    with pytest.raises(ValueError, match="levels"):
+        LevelInputProjection([16, 32], 16, 4)([torch.zeros(1, 16, 2, 3)])

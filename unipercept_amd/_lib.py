@@ -10,7 +10,7 @@ from pathlib import Path
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("MSDA_LIBRARY", _PKG / "libmsda.so"))
 
-ABI_VERSION = 8
+ABI_VERSION = 9
 
 # dtype codes of include/msda.h
 F32, F64, BF16, F16 = 0, 1, 2, 3
@@ -24,6 +24,7 @@ FLAG_RAW_POINTS = 64
 FLAG_BINNED = 128
 FLAG_BIN_ONLY = 256
 SAMPLE_BILINEAR, SAMPLE_NEAREST = 0, 1
+ACT_NONE, ACT_RELU, ACT_SILU, ACT_GELU = 0, 1, 2, 3
 
 # every symbol include/msda.h declares
 EXPORTS = (
@@ -43,6 +44,14 @@ EXPORTS = (
     "msda_point_sample_forward",
     "msda_point_sample_backward",
     "msda_point_sample_workspace_bytes",
+    "msda_dropout_forward",
+    "msda_dropout_backward",
+    "msda_dropout_add_norm_forward",
+    "msda_dropout_add_norm_workspace_bytes",
+    "msda_dropout_add_norm_backward",
+    "msda_group_norm_forward",
+    "msda_group_norm_workspace_bytes",
+    "msda_group_norm_backward",
 )
 
 _lock = threading.Lock()
@@ -92,6 +101,32 @@ def _declare(lib: ctypes.CDLL) -> None:
     lib.msda_point_sample_backward.argtypes = [c_vp] * 6 + [c_sz] + [c_int] * 8 + [c_vp]
     lib.msda_point_sample_workspace_bytes.restype = c_sz
     lib.msda_point_sample_workspace_bytes.argtypes = [c_int] * 6
+
+    c_i64, c_dbl = ctypes.c_int64, ctypes.c_double
+    lib.msda_dropout_forward.restype = c_int
+    lib.msda_dropout_forward.argtypes = [c_vp] * 3 + [c_i64, c_dbl] + [c_int] * 3 + [c_vp]
+    lib.msda_dropout_backward.restype = c_int
+    lib.msda_dropout_backward.argtypes = [c_vp] * 4 + [c_i64, c_dbl] + [c_int] * 3 + [c_vp]
+    lib.msda_dropout_add_norm_forward.restype = c_int
+    lib.msda_dropout_add_norm_forward.argtypes = (
+        [c_vp] * 8 + [c_i64, c_int, c_dbl, c_int, c_dbl] + [c_int] * 3 + [c_vp]
+    )
+    lib.msda_dropout_add_norm_workspace_bytes.restype = c_sz
+    lib.msda_dropout_add_norm_workspace_bytes.argtypes = [c_i64] + [c_int] * 3
+    lib.msda_dropout_add_norm_backward.restype = c_int
+    lib.msda_dropout_add_norm_backward.argtypes = (
+        [c_vp] * 11 + [c_sz, c_vp, c_i64, c_int, c_dbl] + [c_int] * 4 + [c_vp]
+    )
+    lib.msda_group_norm_forward.restype = c_int
+    lib.msda_group_norm_forward.argtypes = (
+        [c_vp] * 7 + [c_sz, c_vp] + [c_int] * 6 + [c_dbl] + [c_int] * 3 + [c_vp]
+    )
+    lib.msda_group_norm_workspace_bytes.restype = c_sz
+    lib.msda_group_norm_workspace_bytes.argtypes = [c_vp] + [c_int] * 7
+    lib.msda_group_norm_backward.restype = c_int
+    lib.msda_group_norm_backward.argtypes = (
+        [c_vp] * 10 + [c_sz, c_vp] + [c_int] * 9 + [c_vp]
+    )
 
 
 def load() -> ctypes.CDLL:

@@ -5,6 +5,7 @@
 
 #include <mutex>
 
+#include "msda_epilogue.h"
 #include "msda_generic.h"
 #include "msda_points.h"
 #include "msda_sample.h"
@@ -14,19 +15,7 @@ namespace {
 
 using namespace msda;
 
-constexpr int kAbiVersion = 8;
-
-inline size_t elem_size(int dtype) {
-  switch (dtype) {
-    case MSDA_F32: return 4;
-    case MSDA_F64: return 8;
-    case MSDA_BF16:
-    case MSDA_F16: return 2;
-    default: return 0;
-  }
-}
-
-inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
+constexpr int kAbiVersion = 9;
 
 inline int check_common(int N, int S, int M, int D, int Lq, int L, int P, int dtype_val,
                         int dtype_loc) {

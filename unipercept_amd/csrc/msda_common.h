@@ -7,7 +7,22 @@
 #include <tuple>
 #include <utility>
 
+#include "../../include/msda.h"
+
 namespace msda {
+
+// ---- arguments ---------------------------------------------------------------------------------
+inline size_t elem_size(int dtype) {
+  switch (dtype) {
+    case MSDA_F32: return 4;
+    case MSDA_F64: return 8;
+    case MSDA_BF16:
+    case MSDA_F16: return 2;
+    default: return 0;
+  }
+}
+
+inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 
 // ---- kernel launches ---------------------------------------------------------------------------
 // Launches through hipLaunchKernel and keeps ITS return code: the status a call reports is that

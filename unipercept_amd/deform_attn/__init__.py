@@ -3,7 +3,9 @@
 Exports what the reference's test imports from that package
 (tests/unipercept/nn/layers/test_nn_layers_deform_attn.py:6-10): ``MultiScaleDeformAttnFunction``,
 ``MultiScaleFlashAttnFunction`` and ``reference``; plus the functional alias ``ms_deform_attn``, the
-``MSDeformAttn`` layer and ``SamplingPointsFunction`` (the layer's fused point epilogue).
+``MSDeformAttn`` layer and ``SamplingPointsFunction`` (the layer's fused point epilogue).  The
+operators around the attention (``counter_dropout``, ``dropout_add_layer_norm``,
+``level_group_norm``) have no counterpart there.
 """
 
 from . import reference
@@ -14,16 +16,24 @@ from ._function import (
     ms_deform_attn,
 )
 from .encoder import (
+    LevelInputProjection,
     MSDeformAttnEncoder,
     MSDeformAttnEncoderLayer,
     encoder_reference_points,
     flatten_levels,
     sine_position_embedding,
 )
+from .epilogue import (
+    counter_dropout,
+    dropout_add_layer_norm,
+    level_group_norm,
+    new_rng_state,
+)
 from .layer import MSDeformAttn
 
 __all__ = [
     "MSDeformAttn",
+    "LevelInputProjection",
     "MSDeformAttnEncoder",
     "MSDeformAttnEncoderLayer",
     "encoder_reference_points",
@@ -32,6 +42,10 @@ __all__ = [
     "MultiScaleDeformAttnFunction",
     "MultiScaleFlashAttnFunction",
     "SamplingPointsFunction",
+    "counter_dropout",
+    "dropout_add_layer_norm",
+    "level_group_norm",
+    "new_rng_state",
     "ms_deform_attn",
     "reference",
 ]

@@ -6,7 +6,8 @@ Mask2Former convention: per layer ``x = LN(x + MSDeformAttn(x + pos, ref, x))`` 
 ``x = LN(x + FFN(x))``, reference points at the pixel centres of every level, sine position
 embeddings as in the reference's ``TrigonometricEmbed2d``
 (sources/unipercept/nn/layers/position.py:63-83,94-122).  Everything here is PyTorch-ROCm
-plumbing (hipBLASLt GEMMs, LayerNorm); the sampling itself runs in the HIP kernels.
+plumbing (hipBLASLt GEMMs, LayerNorm); the sampling itself runs in the HIP kernels, and so does all
+that stands between the GEMMs with ``fused_epilogues`` and in ``LevelInputProjection``.
 """
 
 from __future__ import annotations
@@ -16,6 +17,7 @@ import math
 import torch
 from torch import nn
 
+from .epilogue import counter_dropout, dropout_add_layer_norm, level_group_norm, new_rng_state
 from .layer import MSDeformAttn, token_linear
 
 
@@ -84,6 +86,14 @@ def encoder_reference_points(
 
 
 class MSDeformAttnEncoderLayer(nn.Module):
+    """``fused_epilogues``: dropout, the residual sums, the layer norms and the ReLU run in the HIP
+    kernels of ``epilogue`` (ROCm tensors only): ``dropout_add_layer_norm`` behind the attention and
+    behind the feed-forward network, ``counter_dropout`` on its hidden tensor.  Parameters and state
+    dicts are the same; dropout masks come from ``rng_state`` (see ``forward``)."""
+
+    # uses of one rng_state in a layer: behind the attention, the hidden tensor, behind the network
+    RNG_SITES = 3
+
     def __init__(
         self,
         d_model: int = 256,
@@ -92,8 +102,10 @@ class MSDeformAttnEncoderLayer(nn.Module):
         n_levels: int = 3,
         n_heads: int = 8,
         n_points: int = 4,
+        fused_epilogues: bool = False,
     ):
         super().__init__()
+        self.fused_epilogues = fused_epilogues
         self.self_attn = MSDeformAttn(d_model, n_levels, n_heads, n_points)
         self.norm1 = nn.LayerNorm(d_model)
         self.linear1 = nn.Linear(d_model, d_ffn)
@@ -109,15 +121,39 @@ class MSDeformAttnEncoderLayer(nn.Module):
         spatial_shapes: torch.Tensor,
         level_start_index: torch.Tensor,
         padding_mask: torch.Tensor | None = None,
+        rng_state: torch.Tensor | None = None,
+        rng_site: int = 0,
     ) -> torch.Tensor:
+        """``rng_state``, ``rng_site`` (with ``fused_epilogues``): the state and the first of
+        ``RNG_SITES`` sites of the dropout masks; without a state one is drawn from torch's
+        generator when dropout is active."""
         query = src if pos is None else src + pos
         attn = self.self_attn(
             query, reference_points, src, spatial_shapes, level_start_index, padding_mask
         )
+        if self.fused_epilogues:
+            return self._fused_rest(src, attn, rng_state, rng_site)
         src = self.norm1(src + self.dropout(attn))
         hidden = torch.relu(token_linear(src, self.linear1.weight, self.linear1.bias))
         ffn = token_linear(self.dropout(hidden), self.linear2.weight, self.linear2.bias)
         return self.norm2(src + self.dropout(ffn))
+
+    def _fused_rest(self, src, attn, rng_state, rng_site):
+        p = self.dropout.p if self.training else 0.0
+        if p > 0.0 and rng_state is None:
+            rng_state = new_rng_state(src.device)
+        if torch.is_autocast_enabled("cuda") and src.dtype in (torch.bfloat16, torch.float16):
+            src = src.float()  # autocast keeps the normalised stream in fp32
+        norm1, norm2 = self.norm1, self.norm2
+        src = dropout_add_layer_norm(
+            attn, src, norm1.weight, norm1.bias, p, rng_state, rng_site, norm1.eps
+        )
+        hidden = token_linear(src, self.linear1.weight, self.linear1.bias)
+        hidden = counter_dropout(hidden, p, rng_state, rng_site + 1, "relu")
+        ffn = token_linear(hidden, self.linear2.weight, self.linear2.bias)
+        return dropout_add_layer_norm(
+            ffn, src, norm2.weight, norm2.bias, p, rng_state, rng_site + 2, norm2.eps
+        )
 
 
 class MSDeformAttnEncoder(nn.Module):
@@ -145,8 +181,15 @@ class MSDeformAttnEncoder(nn.Module):
         if ref.shape[0] != src.shape[0]:
             ref = ref.expand(src.shape[0], -1, -1, -1)
         ref = ref.contiguous()
-        for layer in self.layers:
-            src = layer(src, pos, ref, spatial_shapes, level_start_index, padding_mask)
+        # one state for the dropout masks of the stack, sites of its own for every fused layer
+        rng_state = None
+        for i, layer in enumerate(self.layers):
+            args = (src, pos, ref, spatial_shapes, level_start_index, padding_mask)
+            if getattr(layer, "fused_epilogues", False) and layer.training and layer.dropout.p > 0.0:
+                if rng_state is None:
+                    rng_state = new_rng_state(src.device)
+                args += (rng_state, i * MSDeformAttnEncoderLayer.RNG_SITES)
+            src = layer(*args)
         return src
 
 
@@ -172,3 +215,47 @@ def flatten_levels(features, position_feats: int | None = None):
             dim=0,
         )[None].expand(src.shape[0], -1, -1)
     return src, spatial_shapes, level_start_index, shapes, pos
+
+
+class LevelInputProjection(nn.Module):
+    """Input projections of a pixel decoder: for every level a 1 x 1 convolution to ``d_model``
+    channels and a group norm (with an optional activation), flattened to tokens.
+
+    ``forward(features)`` takes the (N, C_l, H_l, W_l) maps and returns what ``flatten_levels``
+    returns for the projected maps.  The convolutions run as token GEMMs on the channels-last maps,
+    the norms of all levels as one ``level_group_norm`` over the flattened pyramid (parameters
+    ``norm_weight`` and ``norm_bias`` (L, d_model), one set a level); ROCm tensors only."""
+
+    def __init__(
+        self,
+        in_channels,
+        d_model: int = 256,
+        num_groups: int = 32,
+        activation: str = "none",
+        eps: float = 1e-5,
+    ):
+        super().__init__()
+        self.projections = nn.ModuleList(nn.Linear(int(c), d_model) for c in in_channels)
+        if d_model % num_groups != 0:
+            raise ValueError(f"d_model ({d_model}) must be divisible by num_groups ({num_groups})")
+        self.norm_weight = nn.Parameter(torch.ones(len(self.projections), d_model))
+        self.norm_bias = nn.Parameter(torch.zeros(len(self.projections), d_model))
+        self.num_groups = num_groups
+        self.activation = activation
+        self.eps = eps
+        for proj in self.projections:
+            nn.init.xavier_uniform_(proj.weight)
+            nn.init.zeros_(proj.bias)
+
+    def forward(self, features, position_feats: int | None = None):
+        if len(features) != len(self.projections):
+            raise ValueError(f"expected {len(self.projections)} levels, got {len(features)}")
+        maps = []
+        for f, proj in zip(features, self.projections):
+            tokens = token_linear(f.permute(0, 2, 3, 1), proj.weight, proj.bias)
+            maps.append(tokens.permute(0, 3, 1, 2))  # a view, as flatten_levels takes it
+        src, spatial_shapes, level_start_index, shapes, pos = flatten_levels(maps, position_feats)
+        src = level_group_norm(
+            src, self.norm_weight, self.norm_bias, self.num_groups, shapes, self.eps, self.activation
+        )
+        return src, spatial_shapes, level_start_index, shapes, pos
