@@ -30,8 +30,22 @@ def hip_command(out: Path) -> list[str]:
     ]
 
 
+def torch_ops_command(out: Path) -> list[str]:
+    """The torch operators over the library: host code only, against the installed PyTorch-ROCm."""
+    from torch.utils import cpp_extension
+
+    flags = ["-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM"]
+    includes = [f for d in cpp_extension.include_paths("cuda") for f in ("-isystem", d)]
+    libs = [f"-L{d}" for d in cpp_extension.library_paths("cuda")]
+    return [
+        os.environ.get("CXX", "g++"), *flags, *includes, "-o", str(out),
+        str(ROOT / "unipercept_amd" / "torch_ops" / "epilogue.cpp"), *libs,
+        "-ltorch_cpu", "-lc10", "-lc10_hip",
+    ]
+
+
 class build_hip(Command):
-    description = "compile unipercept_amd/libmsda.so with hipcc for gfx950"
+    description = "compile libmsda.so with hipcc for gfx950, and libmsda_torch.so over it"
     user_options = [("force", "f", "rebuild even when the library is newer than its sources")]
 
     def initialize_options(self):
@@ -45,8 +59,16 @@ class build_hip(Command):
         deps = list((ROOT / "unipercept_amd" / "csrc").glob("*")) + [ROOT / "include" / "msda.h"]
         if not self.force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
             print(f"{out} is up to date")
+        else:
+            cmd = hip_command(out)
+            print(" ".join(cmd))
+            subprocess.run(cmd, check=True)
+        out = ROOT / "unipercept_amd" / "libmsda_torch.so"
+        deps = [*(ROOT / "unipercept_amd" / "torch_ops").glob("*.cpp"), ROOT / "include" / "msda.h"]
+        if not self.force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
+            print(f"{out} is up to date")
             return
-        cmd = hip_command(out)
+        cmd = torch_ops_command(out)
         print(" ".join(cmd))
         subprocess.run(cmd, check=True)
 

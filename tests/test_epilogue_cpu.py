@@ -22,7 +22,7 @@ from unipercept_amd.deform_attn import (
     level_group_norm,
     new_rng_state,
 )
-from unipercept_amd.deform_attn import _epilogue_ops as ops
+from unipercept_amd.deform_attn import epilogue
 
 FAKE = 0x1000  # never dereferenced: every call below fails validation first
 
@@ -209,12 +209,47 @@ def test_shapes_and_types_without_running():
     assert new_rng_state("cpu").shape == (2,) and new_rng_state("cpu").dtype == torch.int64
 
 
-def test_level_rows_come_from_lists_tensors_and_plain_shapes():
-    x = meta(2, 20, 8)
-    assert ops.level_rows(x, [(4, 4), (2, 2)]) == [16, 4]
-    assert ops.level_rows(x, torch.tensor([[4, 4], [2, 2]])) == [16, 4]
-    assert ops.level_rows(meta(2, 4, 5, 8), None) == [20]
-    assert ops.level_rows(meta(2, 8), None) == [1]
+def test_level_rows_come_from_lists_and_tensors():
+    assert epilogue.level_rows([(4, 4), (2, 2)]) == [16, 4]
+    assert epilogue.level_rows(torch.tensor([[4, 4], [2, 2]])) == [16, 4]
+    assert level_group_norm(meta(2, 4, 5, 8), meta(8), meta(8), 4).shape == (2, 4, 5, 8)
+    assert level_group_norm(meta(2, 8), meta(8), meta(8), 4).shape == (2, 8)
+    with pytest.raises(ValueError):
+        level_group_norm(meta(2, 4, 8), meta(8), meta(8), 4, [])
+
+
+def test_gradients_have_shapes_without_running():
+    """The operators' graphs on the meta device: types and shapes of every gradient."""
+    x = meta(2, 20, 8, dtype=BF).requires_grad_(True)
+    res, w, b = (t.requires_grad_(True) for t in (meta(2, 20, 8), meta(8), meta(8)))
+    y = dropout_add_layer_norm(counter_dropout(x, 0.1, STATE, 1, "relu"), res, w, b, 0.1, STATE)
+    y = level_group_norm(y, w, b, 4, [(4, 4), (2, 2)], activation="gelu")
+    grads = torch.autograd.grad(y, (x, res, w, b), torch.empty_like(y))
+    assert [g.dtype for g in grads] == [BF, torch.float32, torch.float32, torch.float32]
+    assert [g.shape for g in grads] == [t.shape for t in (x, res, w, b)]
+
+
+def test_torch_operators_are_built_and_loud_when_missing(monkeypatch, tmp_path):
+    assert _lib.torch_ops() is torch.ops.unipercept
+    monkeypatch.setattr(_lib, "_torch_ops", None)
+    monkeypatch.setattr(_lib, "TORCH_LIB_PATH", tmp_path / "libmsda_torch.so")
+    with pytest.raises(_lib.MsdaLibraryError):
+        counter_dropout(meta(4), 0.1, STATE)
+
+
+def test_packaging_builds_the_same_torch_operators():
+    import importlib.util
+    from pathlib import Path
+
+    import __graft_entry__ as entry
+
+    root = Path(entry.__file__).resolve().parent
+    spec = importlib.util.spec_from_file_location("_setup_under_test", root / "setup.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    out = root / "unipercept_amd" / "libmsda_torch.so"
+    assert mod.torch_ops_command(out) == entry.torch_ops_command(out)
+    assert entry.build_torch_ops() == out
 
 
 # ---- argument errors of the C ABI -------------------------------------------------------------------

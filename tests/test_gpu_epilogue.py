@@ -741,3 +741,25 @@ def test_masks_of_a_state_from_torchs_generator():
     kept = (y != 0).double().mean().item()
     # five standard deviations of a binomial share
     assert abs(kept - (1 - round(6553.6) / 65536)) < 5 * (0.09 / (1 << 20)) ** 0.5
+
+
+def test_compiled_graphs_hold_the_operators():
+    """torch.compile (tracing only, eager kernels): forward and backward as in eager mode."""
+    calls, state = _calls()
+    w, b = torch.ones(64, device="cuda", requires_grad=True), torch.zeros(64, device="cuda", requires_grad=True)
+    x, res = normal((2, 20, 64), F32, 1).cuda(), normal((2, 20, 64), F32, 2).cuda()
+
+    def net(x, res, w, b, state):
+        h = counter_dropout(x, 0.2, state, 1, "relu")
+        h = dropout_add_layer_norm(h, res, w, b, 0.2, state, 2)
+        return level_group_norm(h, w, b, 8, [(4, 4), (2, 2)], activation="silu")
+
+    def grads(f):
+        xs = x.clone().requires_grad_(True)
+        out = f(xs, res, w, b, state)
+        return [out.detach(), *torch.autograd.grad(out.square().sum(), (xs, w, b))]
+
+    want = grads(net)
+    got = grads(torch.compile(net, backend="aot_eager", fullgraph=True))
+    for a, c in zip(got, want):
+        assert torch.equal(a, c)

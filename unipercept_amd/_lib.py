@@ -9,6 +9,8 @@ from pathlib import Path
 
 _PKG = Path(__file__).resolve().parent
 LIB_PATH = Path(os.environ.get("MSDA_LIBRARY", _PKG / "libmsda.so"))
+# torch operators over that library (torch_ops/), for calls too short for a Python layer
+TORCH_LIB_PATH = _PKG / "libmsda_torch.so"
 
 ABI_VERSION = 9
 
@@ -56,6 +58,7 @@ EXPORTS = (
 
 _lock = threading.Lock()
 _lib = None
+_torch_ops = None
 
 
 class MsdaLibraryError(RuntimeError):
@@ -151,6 +154,28 @@ def load() -> ctypes.CDLL:
                     )
                 _lib = lib
     return _lib
+
+
+def torch_ops():
+    """``torch.ops.unipercept`` with the operators of ``libmsda_torch.so`` in it; raises if that
+    library has not been built."""
+    global _torch_ops
+    if _torch_ops is None:
+        import torch
+
+        load()
+        with _lock:
+            if _torch_ops is None:
+                if not TORCH_LIB_PATH.exists():
+                    raise MsdaLibraryError(
+                        f"{TORCH_LIB_PATH} not found: build it with `python -c 'import __graft_entry__ "
+                        "as g; g.build()'`. There is no fallback."
+                    )
+                # the operators take the C entry points from the library that is loaded already
+                ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
+                torch.ops.load_library(str(TORCH_LIB_PATH))
+                _torch_ops = torch.ops.unipercept
+    return _torch_ops
 
 
 def check(code: int, what: str) -> None:

@@ -14,9 +14,8 @@ run.  ``MSDeformAttnEncoderLayer(fused_epilogues=True)`` and ``LevelInputProject
 from __future__ import annotations
 
 import torch
-from torch.autograd.function import once_differentiable
 
-from . import _epilogue_ops as ops
+from .. import _lib
 
 
 def new_rng_state(device, generator: torch.Generator | None = None) -> torch.Tensor:
@@ -28,92 +27,18 @@ def new_rng_state(device, generator: torch.Generator | None = None) -> torch.Ten
     )
 
 
-class CounterDropoutFunction(torch.autograd.Function):
-    """``apply(x, rng_state, p, site, activation)``.  Saves the output with "relu" (the next layer
-    keeps it anyway) and only the state otherwise."""
-
-    @staticmethod
-    def forward(ctx, x, rng_state, p, site, activation):
-        out = ops.counter_dropout_fwd(x, rng_state, p, site, activation)
-        if activation == "relu":
-            ctx.save_for_backward(out, None)
-        else:
-            ctx.save_for_backward(None, rng_state)
-        ctx.args = (p, site, activation)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        out, rng_state = ctx.saved_tensors
-        p, site, activation = ctx.args
-        grad = ops.counter_dropout_bwd(grad_output, out, rng_state, p, site, activation)
-        return grad, None, None, None, None
-
-
-class DropoutAddLayerNormFunction(torch.autograd.Function):
-    """``apply(x, residual, weight, bias, rng_state, p, site, eps)``.  Saves the inputs and two values
-    a row; the sum that is normalised is computed again in the backward."""
-
-    @staticmethod
-    def forward(ctx, x, residual, weight, bias, rng_state, p, site, eps):
-        out, mean, rstd = ops.dropout_add_norm_fwd(
-            x, residual, weight, bias, rng_state, p, site, eps, True
-        )
-        ctx.save_for_backward(x, residual, weight, mean, rstd, rng_state)
-        ctx.args = (p, site)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        x, residual, weight, mean, rstd, rng_state = ctx.saved_tensors
-        p, site = ctx.args
-        need_x, need_residual, need_weight, need_bias = ctx.needs_input_grad[:4]
-        # nothing dropped and one type: both gradients are the same tensor
-        shared = p == 0.0 and x.dtype == residual.dtype
-        grad_x, grad_residual, grad_weight, grad_bias = ops.dropout_add_norm_bwd(
-            grad_output, x, residual, weight, mean, rstd, rng_state, p, site,
-            need_x and not shared, need_residual or (shared and need_x), need_weight or need_bias,
-        )
-        if shared:
-            grad_x = grad_residual
-        return (
-            grad_x if need_x else None, grad_residual if need_residual else None,
-            grad_weight if need_weight else None, grad_bias if need_bias else None,
-            None, None, None, None,
-        )
-
-
-class LevelGroupNormFunction(torch.autograd.Function):
-    """``apply(x, weight, bias, num_groups, rows, eps, activation)``, `rows` the row count of every
-    level.  Saves the inputs and two values a (sample, level, group)."""
-
-    @staticmethod
-    def forward(ctx, x, weight, bias, num_groups, rows, eps, activation):
-        out, mean, rstd = ops.level_group_norm_fwd(
-            x, weight, bias, num_groups, rows, eps, activation, True
-        )
-        ctx.save_for_backward(x, weight, bias, mean, rstd)
-        ctx.args = (num_groups, rows, activation)
-        return out
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad_output):
-        x, weight, bias, mean, rstd = ctx.saved_tensors
-        need_x, need_weight, need_bias = ctx.needs_input_grad[:3]
-        grad_x, grad_weight, grad_bias = ops.level_group_norm_bwd(
-            grad_output, x, weight, bias, mean, rstd, *ctx.args, need_x, need_weight or need_bias
-        )
-        return (
-            grad_x if need_x else None, grad_weight if need_weight else None,
-            grad_bias if need_bias else None, None, None, None, None,
-        )
-
-
-def _grad_wanted(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors)
+def level_rows(spatial_shapes) -> list[int]:
+    """Rows of every level from its (H, W) pairs."""
+    if isinstance(spatial_shapes, torch.Tensor):
+        spatial_shapes = spatial_shapes.tolist()  # a device read; pass a list to avoid it
+    rows = []
+    for h, w in spatial_shapes:
+        if h < 1 or w < 1:
+            raise ValueError(f"level_group_norm: spatial_shapes must be positive, got {list(spatial_shapes)}")
+        rows.append(int(h) * int(w))
+    if not rows:
+        raise ValueError("level_group_norm: spatial_shapes is empty")
+    return rows
 
 
 def counter_dropout(
@@ -133,14 +58,7 @@ def counter_dropout(
     the kernel runs, so a captured graph draws new masks if the caller changes it between replays;
     do not change it between a forward and its backward.  Without anything to do (p = 0, no
     activation) x itself is returned."""
-    ops.check_dropout(x, p, rng_state, site, activation)
-    if p == 0.0:
-        if activation == "none":
-            return x
-        rng_state = None
-    if _grad_wanted(x):
-        return CounterDropoutFunction.apply(x, rng_state, p, site, activation)
-    return ops.counter_dropout_fwd(x, rng_state, p, site, activation)
+    return _lib.torch_ops().counter_dropout(x, p, rng_state, site, activation)
 
 
 def dropout_add_layer_norm(
@@ -159,12 +77,7 @@ def dropout_add_layer_norm(
     ``residual`` has x's shape and dtype, or float32 next to a 16-bit x (autocast); ``weight`` and
     ``bias`` have residual's dtype or, next to a 16-bit x, float32.  Rows of up to 16 KiB in
     ``residual``'s dtype.  For the mask see ``counter_dropout``."""
-    ops.check_add_norm(x, residual, weight, bias, p, rng_state, site, eps)
-    if p == 0.0:
-        rng_state = None
-    if _grad_wanted(x, residual, weight, bias):
-        return DropoutAddLayerNormFunction.apply(x, residual, weight, bias, rng_state, p, site, eps)
-    return ops.dropout_add_norm_fwd(x, residual, weight, bias, rng_state, p, site, eps, False)[0]
+    return _lib.torch_ops().dropout_add_layer_norm(x, residual, weight, bias, p, rng_state, site, eps)
 
 
 def level_group_norm(
@@ -185,8 +98,11 @@ def level_group_norm(
     (C,) or, one set a level, (L, C), in x's dtype or float32 next to 16 bits.  The normal result for
     a level is that of ``torch.nn.functional.group_norm`` on its (N, C, H, W) map.  Rows (C channels)
     of up to 16 KiB."""
-    rows = ops.level_rows(x, spatial_shapes)
-    ops.check_group_norm(x, weight, bias, num_groups, rows, eps, activation)
-    if _grad_wanted(x, weight, bias):
-        return LevelGroupNormFunction.apply(x, weight, bias, num_groups, rows, eps, activation)
-    return ops.level_group_norm_fwd(x, weight, bias, num_groups, rows, eps, activation, False)[0]
+    rows = []
+    if spatial_shapes is not None:
+        if x.dim() != 3:
+            raise ValueError(
+                f"level_group_norm: with spatial_shapes x must be (N, S, C), got {tuple(x.shape)}"
+            )
+        rows = level_rows(spatial_shapes)
+    return _lib.torch_ops().level_group_norm(x, weight, bias, num_groups, rows, eps, activation)
