@@ -186,6 +186,8 @@ GROUP = dict(x=meta(2, 20, 8), weight=meta(8), bias=meta(8), num_groups=4)
         (dict(eps=-1.0), ValueError),
         (dict(x=meta(1, 2, 8200, dtype=BF), weight=meta(8200), bias=meta(8200)), ValueError),
         (dict(x=meta(2, 20, 8, dtype=torch.int64)), TypeError),
+        (dict(x=meta(2**21 + 1, 1, 8)), ValueError),
+        (dict(x=meta(2**20 + 1, 2, 8), spatial_shapes=[(1, 1), (1, 1)]), ValueError),
     ],
 )
 def test_group_norm_refusals(change, exc):
@@ -302,9 +304,9 @@ def test_abi_add_norm_errors():
         assert call(dx=1, dr=1, dp=1, c=2049) == -2  # 16 KiB of the residual's type
     assert fwd(eps=-1.0) == -2 and fwd(eps=float("nan")) == -2
     assert bwd(ws=None) == -5 and bwd(ws=FAKE + 4) == -5 and bwd(nbytes=need(4, 8, 0, 0) - 1) == -5
-    # sums of two per column and workgroup; at most 1024 workgroups
-    assert need(4, 8, 0, 0) == 4 * 2 * 8 * 4 and need(10**6, 256, 2, 0) == 1024 * 2 * 256 * 4
-    assert need(4, 8, 1, 1) == 4 * 2 * 8 * 8 and need(0, 8, 0, 0) == 0 and need(4, 8, 0, 2) == 0
+    # two sums per column and workgroup; 512 threads take 64 rows of 256 fp32 columns
+    assert need(4, 8, 0, 0) == 2 * 8 * 4 and need(10**6, 256, 2, 0) == 15625 * 2 * 256 * 4
+    assert need(4, 8, 1, 1) == 2 * 8 * 8 and need(0, 8, 0, 0) == 0 and need(4, 8, 0, 2) == 0
 
 
 def test_abi_group_norm_errors():
@@ -334,7 +336,7 @@ def test_abi_group_norm_errors():
         assert call(g=3) == -2 and call(pl=3) == -2 and call(pl=0) == -2
         assert call(rows=(16, 5)) == -2 and call(rows=(21, -1)) == -2 and call(rows=(20, 0)) == -2
         assert call(rows=(1,) * 17, l=17, s=17) == -7
-        assert call(c=4100) == -2 and call(n=1 << 30) == -2
+        assert call(c=4100) == -2 and call(n=1 << 30) == -2 and call(n=(1 << 20) + 1) == -2
         assert call(dtype=9) == -3 and call(act=4) == -3 and call(act=-1) == -3 and call(dp=2) == -3
         assert call(dtype=1, dp=0) == -3 and call(dtype=2, dp=3) == -3
         assert call(x=FAKE + 2) == -4 and call(mean=FAKE + 2) == -4

@@ -68,8 +68,10 @@ __device__ __forceinline__ uint32_t keep_bits(const DropKey& key, uint64_t first
   return VE == 8 && ALIGNED ? bits : bits >> at;
 }
 
-// One generator block (8 elements) per thread and step.  RELU: y = max(x, 0) first (NaN stays);
-// a dropped element is 0 whatever x holds.
+// One vector of 16 bytes per thread and step: with fp32 two lanes share a generator block and both
+// compute it, which leaves the arithmetic per byte that of the 16-bit types (two vectors a lane
+// instead leave every access half a line: 54 MB in 44 us against 20).  RELU: y = max(x, 0) first
+// (NaN stays); a dropped element is 0 whatever x holds.
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ out,
                                                       const int64_t* __restrict__ rng_state,
@@ -77,37 +79,32 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
                                                       typename Elem<T>::compute_t scale,
                                                       uint32_t site) {
   using ct = typename Elem<T>::compute_t;
-  constexpr int VE = 16 / sizeof(T), PARTS = 8 / VE;
+  constexpr int VE = 16 / sizeof(T);
   const DropKey key = DROP ? load_drop_key(rng_state) : DropKey{};
-  const int64_t blocks = (numel + 7) >> 3;
-  for (int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; b < blocks;
+  const int64_t vecs = (numel + VE - 1) / VE;
+  for (int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; b < vecs;
        b += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t first = b * 8;
-    const int64_t left = numel - first;
-    Pack<T, VE> in[PARTS];
-#pragma unroll
-    for (int k = 0; k < PARTS; ++k) {
-      const int64_t n = left - k * VE;
-      if (n > 0) {
-        in[k].load(x + first + k * VE, n < VE ? static_cast<int>(n) : VE);
-      } else {
-        in[k].zero();
-      }
+    const int64_t first = b * VE, left = numel - first;
+    Pack<T, VE> p;
+    if (left >= VE) {
+      p.template load<true>(x + first);
+    } else {
+      p.load_part(x + first, static_cast<int>(left));
     }
-    const uint32_t keep = DROP ? keep_block(key, static_cast<uint32_t>(b), site, threshold) : 0xFFu;
+    const uint32_t keep = DROP ? keep_bits<VE, true>(key, first, site, threshold) : 0xFFu;
+    ct v[VE];
+    p.unpack(v);
 #pragma unroll
-    for (int k = 0; k < PARTS; ++k) {
-      ct v[VE];
-      in[k].unpack(v);
-#pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        bool on = (keep >> (k * VE + i)) & 1u;
-        if (RELU) on = on && !(v[i] <= ct(0));
-        v[i] = on ? v[i] * scale : ct(0);
-      }
-      in[k].pack(v);
-      const int64_t n = left - k * VE;
-      if (n > 0) in[k].store(out + first + k * VE, n < VE ? static_cast<int>(n) : VE);
+    for (int i = 0; i < VE; ++i) {
+      bool on = (keep >> i) & 1u;
+      if (RELU) on = on && !(v[i] <= ct(0));
+      v[i] = on ? v[i] * scale : ct(0);
+    }
+    p.pack(v);
+    if (left >= VE) {
+      p.template store<true>(out + first);
+    } else {
+      p.store_part(out + first, static_cast<int>(left));
     }
   }
 }
@@ -123,18 +120,26 @@ __global__ __launch_bounds__(256) void dropout_relu_bwd_kernel(
   const int64_t vecs = (numel + VE - 1) / VE;
   for (int64_t b = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; b < vecs;
        b += static_cast<int64_t>(gridDim.x) * 256) {
-    const int64_t left = numel - b * VE;
-    const int n = left < VE ? static_cast<int>(left) : VE;
+    const int64_t first = b * VE, left = numel - first;
     Pack<T, VE> g, o;
-    g.load(grad_out + b * VE, n);
-    o.load(y + b * VE, n);
+    if (left >= VE) {
+      g.template load<true>(grad_out + first);
+      o.template load<true>(y + first);
+    } else {
+      g.load_part(grad_out + first, static_cast<int>(left));
+      o.load_part(y + first, static_cast<int>(left));
+    }
     ct gv[VE], ov[VE];
     g.unpack(gv);
     o.unpack(ov);
 #pragma unroll
     for (int i = 0; i < VE; ++i) gv[i] = ov[i] <= ct(0) ? ct(0) : gv[i] * scale;
     g.pack(gv);
-    g.store(grad_x + b * VE, n);
+    if (left >= VE) {
+      g.template store<true>(grad_x + first);
+    } else {
+      g.store_part(grad_x + first, static_cast<int>(left));
+    }
   }
 }
 

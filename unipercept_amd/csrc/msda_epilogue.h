@@ -30,11 +30,12 @@ inline bool drop_args(double p, DropArgs* a) {
 
 constexpr int64_t kMaxDropElements = static_cast<int64_t>(1) << 35;  // 32-bit block counter
 
-// Workgroups of a pass over `items` thread steps of 256: enough of them to fill the chip several
-// times over (2048 hold 8 on every CU), each thread looping over what is left.
-inline unsigned pass_grid(int64_t items) {
-  const int64_t blocks = (items + 255) / 256;
-  return static_cast<unsigned>(blocks < 4096 ? blocks : 4096);
+// Workgroups of a pass over `items` steps of `per_block` a workgroup: one step each, so that loads
+// of the next workgroups overlap the stores of the last (a copy of 352 MB runs at 6.7 TB/s so and
+// at 5.8 with 2048 workgroups that loop); more than a launch holds are looped over.
+inline unsigned pass_grid(int64_t items, int per_block) {
+  const int64_t blocks = (items + per_block - 1) / per_block;
+  return static_cast<unsigned>(blocks < (1 << 23) ? blocks : (1 << 23));
 }
 
 template <typename T>
@@ -42,7 +43,8 @@ int dropout_forward(const void* x, void* out, const int64_t* rng_state, int64_t 
                     const DropArgs& d, uint32_t site, bool relu, hipStream_t stream) {
   using ct = typename Elem<T>::compute_t;
   Launches run;
-  const dim3 grid(pass_grid((numel + 7) / 8));
+  constexpr int VE = 16 / sizeof(T);
+  const dim3 grid(pass_grid((numel + VE - 1) / VE, 256));
 #define MSDA_DROP(RELU, DROP)                                                                  \
   run((dropout_kernel<T, RELU, DROP>), grid, dim3(256), 0, stream, static_cast<const T*>(x),   \
       static_cast<T*>(out), rng_state, numel, d.threshold, static_cast<ct>(d.scale), site)
@@ -62,19 +64,10 @@ int dropout_relu_backward(const void* grad_out, const void* out, void* grad_x, i
                           const DropArgs& d, hipStream_t stream) {
   Launches run;
   constexpr int VE = 16 / sizeof(T);
-  run((dropout_relu_bwd_kernel<T>), dim3(pass_grid((numel + VE - 1) / VE)), dim3(256), 0, stream,
+  run((dropout_relu_bwd_kernel<T>), dim3(pass_grid((numel + VE - 1) / VE, 256)), dim3(256), 0, stream,
       static_cast<const T*>(grad_out), static_cast<const T*>(out), static_cast<T*>(grad_x), numel,
       static_cast<typename Elem<T>::compute_t>(d.scale));
   return run.rc;
-}
-
-// ---- column sums --------------------------------------------------------------------------------
-template <typename T>
-void column_sums(Launches& run, const void* partial, void* dst0, void* dst1, const ColumnRuns& runs,
-                 int levels, int C, bool wide, hipStream_t stream) {
-  using ct = typename Elem<T>::compute_t;
-  run((column_sums_kernel<T>), dim3((C + 15) / 16, 2, levels), dim3(1024), 0, stream,
-      static_cast<const ct*>(partial), dst0, dst1, runs, C, wide ? 1 : 0);
 }
 
 // ---- dropout + residual + layer norm ------------------------------------------------------------
@@ -97,15 +90,44 @@ inline int add_norm_check(int64_t rows, int C, double p, int site, int dtype_x, 
   return MSDA_OK;
 }
 
-// workgroups of the backward: each leaves one row of partial parameter gradients
-inline int64_t add_norm_bwd_blocks(int64_t rows) { return rows < 1024 ? rows : 1024; }
+// A team of lanes for a row of `vecs` vectors: the narrowest that covers it.  A wave or less per row
+// needs no barrier, so rows of up to four vectors a lane stay in one wave; longer ones take a
+// workgroup of four waves.
+inline int add_norm_team(int vecs) { return vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 ? 64 : 256; }
+// threads of a workgroup and rows in flight of a team in the backward
+constexpr int add_norm_bwd_threads(int TS) { return TS > 64 ? 256 : 512; }
+constexpr int add_norm_bwd_rows(int NV) { return NV == 1 ? 2 : 1; }
+
+// Steps of a workgroup of the backward (NR rows a team each): up to kBwdTeamRows rows a team where
+// there are many rows, one step where there are few, so that they spread over the chip.  Longer
+// workgroups leave fewer partial rows and run slower (344064 rows of 256 fp32 columns, kernel and
+// column sums: 2 rows a team 320 + 21 us, 4 rows 296 + 15, 8 rows 310 + 14, 16 rows 330 + 9).
+constexpr int kBwdTeamRows = 4;
+struct AddNormGrid {
+  int steps;
+  int64_t blocks;
+};
+inline AddNormGrid add_norm_bwd_grid(int64_t rows, int C, int dtype_res) {
+  const int VE = 16 / static_cast<int>(elem_size(dtype_res)), vecs = (C + VE - 1) / VE;
+  const int TS = add_norm_team(vecs), NR = add_norm_bwd_rows((vecs + TS - 1) / TS);
+  const int64_t per_step = static_cast<int64_t>(add_norm_bwd_threads(TS) / TS) * NR;
+  const int most = kBwdTeamRows / NR;
+  int64_t steps = rows / (per_step * 512);
+  steps = steps < 1 ? 1 : steps > most ? most : steps;
+  while ((rows + per_step * steps - 1) / (per_step * steps) > (1 << 22)) steps *= 2;
+  return {static_cast<int>(steps), (rows + per_step * steps - 1) / (per_step * steps)};
+}
+
+// Partial rows that one workgroup a tile of columns adds up; more are added in segments first (11 MB
+// of partial rows: 14 us in one step, 8 in two; 22 MB: 26 and 15).
+constexpr int kColumnSplit = 1024, kColumnSegments = 16;
 
 struct AddNormCall {
   const void *grad_out, *x, *res, *weight, *bias;
   void *out, *mean, *rstd, *grad_x, *grad_res, *grad_weight, *grad_bias, *partial;
   const int64_t* rng_state;
   int64_t rows;
-  int C;
+  int C, dtype_res;
   DropArgs drop;
   uint32_t site;
   double eps;
@@ -113,56 +135,65 @@ struct AddNormCall {
   hipStream_t stream;
 };
 
-template <typename XT, typename RT, int TS, int NV, bool EVEN>
+template <typename XT, typename RT, int TS, int NV, int MODE>
 int add_norm_launch(const AddNormCall& a, bool backward) {
   using ct = typename Elem<RT>::compute_t;
-  constexpr int TEAMS = 256 / TS;
-  const int64_t need = (a.rows + TEAMS - 1) / TEAMS;
   Launches run;
   if (!backward) {
-    run((add_norm_fwd_kernel<XT, RT, TS, NV, EVEN>),
-        dim3(static_cast<unsigned>(need < 4096 ? need : 4096)), dim3(256), 0, a.stream,
-        static_cast<const XT*>(a.x), static_cast<const RT*>(a.res), a.weight, a.bias,
-        static_cast<RT*>(a.out), static_cast<ct*>(a.mean), static_cast<ct*>(a.rstd), a.rng_state,
-        a.rows, a.C, a.drop.threshold, static_cast<ct>(a.drop.scale), a.site,
+    constexpr int NR = NV == 1 ? 2 : 1;
+    run((add_norm_fwd_kernel<XT, RT, TS, NV, NR, MODE>), dim3(pass_grid(a.rows, 256 / TS * NR)),
+        dim3(256), 0, a.stream, static_cast<const XT*>(a.x), static_cast<const RT*>(a.res), a.weight,
+        a.bias, static_cast<RT*>(a.out), static_cast<ct*>(a.mean), static_cast<ct*>(a.rstd),
+        a.rng_state, a.rows, a.C, a.drop.threshold, static_cast<ct>(a.drop.scale), a.site,
         static_cast<ct>(a.eps), a.wide ? 1 : 0);
     return run.rc;
   }
-  const int64_t most = add_norm_bwd_blocks(a.rows);
-  const int blocks = static_cast<int>(need < most ? need : most);
-  run((add_norm_bwd_kernel<XT, RT, TS, NV, EVEN>), dim3(blocks), dim3(256), 0, a.stream,
+  constexpr int THREADS = add_norm_bwd_threads(TS), NR = add_norm_bwd_rows(NV);
+  const AddNormGrid grid = add_norm_bwd_grid(a.rows, a.C, a.dtype_res);
+  run((add_norm_bwd_kernel<XT, RT, TS, NV, NR, THREADS, MODE>),
+      dim3(static_cast<unsigned>(grid.blocks)), dim3(THREADS), 0, a.stream,
       static_cast<const RT*>(a.grad_out), static_cast<const XT*>(a.x),
       static_cast<const RT*>(a.res), a.weight, static_cast<const ct*>(a.mean),
       static_cast<const ct*>(a.rstd), static_cast<XT*>(a.grad_x), static_cast<RT*>(a.grad_res),
-      static_cast<ct*>(a.partial), a.rng_state, a.rows, a.C, a.drop.threshold,
+      static_cast<ct*>(a.partial), a.rng_state, a.rows, a.C, grid.steps, a.drop.threshold,
       static_cast<ct>(a.drop.scale), a.site, a.wide ? 1 : 0);
   if (a.partial != nullptr) {
-    ColumnRuns runs{};
-    runs.outer = 1;
-    runs.end[0] = blocks;
-    column_sums<RT>(run, a.partial, a.grad_weight, a.grad_bias, runs, 1, a.C, a.wide, a.stream);
+    const dim3 tiles((a.C + 15) / 16, 2, 1);
+    const ct* src = static_cast<const ct*>(a.partial);
+    ct* next = static_cast<ct*>(a.partial) + grid.blocks * 2 * a.C;
+    int total = static_cast<int>(grid.blocks);
+    if (total > kColumnSplit) {
+      run((column_sums_kernel<RT>), dim3(tiles.x, 2, kColumnSegments), dim3(1024), 0, a.stream, src,
+          next, nullptr, nullptr, total, a.C, 1);
+      src = next;
+      total = kColumnSegments;
+    }
+    run((column_sums_kernel<RT>), tiles, dim3(1024), 0, a.stream, src, nullptr, a.grad_weight,
+        a.grad_bias, total, a.C, a.wide ? 1 : 0);
   }
   return run.rc;
 }
 
-// The narrowest team whose lanes cover a row: a wave or less per row needs no barrier; rows of up
-// to four vectors a lane of one wave stay there, longer ones go to the whole workgroup.
-template <typename XT, typename RT, bool EVEN>
+// (team sizes: add_norm_team)
+template <typename XT, typename RT, int MODE>
 int add_norm_width(const AddNormCall& a, bool backward) {
   const int vecs = (a.C + AddNormTypes<XT, RT>::VE - 1) / AddNormTypes<XT, RT>::VE;
-  if (vecs <= 16) return add_norm_launch<XT, RT, 16, 1, EVEN>(a, backward);
-  if (vecs <= 32) return add_norm_launch<XT, RT, 32, 1, EVEN>(a, backward);
-  if (vecs <= 64) return add_norm_launch<XT, RT, 64, 1, EVEN>(a, backward);
-  if (vecs <= 128) return add_norm_launch<XT, RT, 64, 2, EVEN>(a, backward);
-  if (vecs <= 256) return add_norm_launch<XT, RT, 64, 4, EVEN>(a, backward);
-  if (vecs <= 512) return add_norm_launch<XT, RT, 256, 2, EVEN>(a, backward);
-  return add_norm_launch<XT, RT, 256, 4, EVEN>(a, backward);
+  if (vecs <= 16) return add_norm_launch<XT, RT, 16, 1, MODE>(a, backward);
+  if (vecs <= 32) return add_norm_launch<XT, RT, 32, 1, MODE>(a, backward);
+  if (vecs <= 64) return add_norm_launch<XT, RT, 64, 1, MODE>(a, backward);
+  if (vecs <= 128) return add_norm_launch<XT, RT, 64, 2, MODE>(a, backward);
+  if (vecs <= 256) return add_norm_launch<XT, RT, 64, 4, MODE>(a, backward);
+  if (vecs <= 512) return add_norm_launch<XT, RT, 256, 2, MODE>(a, backward);
+  return add_norm_launch<XT, RT, 256, 4, MODE>(a, backward);
 }
 
 template <typename XT, typename RT>
 int add_norm_run(const AddNormCall& a, bool backward) {
-  return a.C % AddNormTypes<XT, RT>::VE == 0 ? add_norm_width<XT, RT, true>(a, backward)
-                                             : add_norm_width<XT, RT, false>(a, backward);
+  switch (row_mode(a.C, AddNormTypes<XT, RT>::VE)) {
+    case kRowEven: return add_norm_width<XT, RT, kRowEven>(a, backward);
+    case kRowOdd: return add_norm_width<XT, RT, kRowOdd>(a, backward);
+    default: return add_norm_launch<XT, RT, 16, 1, kRowShort>(a, backward);
+  }
 }
 
 inline int add_norm_dispatch(const AddNormCall& a, int dtype_x, int dtype_res, bool backward) {
@@ -180,15 +211,29 @@ inline int add_norm_dispatch(const AddNormCall& a, int dtype_x, int dtype_res, b
 
 // ---- group norm ---------------------------------------------------------------------------------
 struct GnPlan {
-  GnLevels lv;
-  int threads, lanes, team_width;
-  int64_t blocks;
+  GnCut sums, writes;  // chunks of the passes that sum and of those that write
+  int param_levels, lanes, tiles;
+  int64_t cells;  // (sample, level, group)
 };
+
+inline void gn_cut(const int64_t* level_rows, int L, int64_t rows_per_chunk, GnCut* cut) {
+  cut->levels = L;
+  cut->rows_per_chunk = static_cast<int>(rows_per_chunk);
+  cut->row_start[0] = cut->chunk_start[0] = 0;
+  for (int l = 0; l < L; ++l) {
+    cut->row_start[l + 1] = cut->row_start[l] + static_cast<int>(level_rows[l]);
+    cut->chunk_start[l + 1] =
+        cut->chunk_start[l] + static_cast<int>((level_rows[l] + rows_per_chunk - 1) / rows_per_chunk);
+  }
+  cut->chunks = cut->chunk_start[L];
+}
 
 inline int gn_plan(const int64_t* level_rows, int N, int S, int C, int G, int L, int param_levels,
                    int activation, int dtype, int dtype_param, GnPlan* plan) {
   if (N < 1 || S < 1 || C < 1 || G < 1 || L < 1 || C % G != 0) return MSDA_ESHAPE;
   if (L > kMaxNormLevels) return MSDA_ELEVELS;
+  // threads of a launch: 32 bits
+  if (static_cast<int64_t>(N) * L * ((G + 31) / 32) > (1 << 21)) return MSDA_ESHAPE;
   if (param_levels != 1 && param_levels != L) return MSDA_ESHAPE;
   const int64_t e = static_cast<int64_t>(elem_size(dtype));
   if (e == 0 || activation < kGnNone || activation > kGnGelu) return MSDA_EDTYPE;
@@ -201,104 +246,125 @@ inline int gn_plan(const int64_t* level_rows, int N, int S, int C, int G, int L,
     longest = level_rows[l] > longest ? level_rows[l] : longest;
   }
   if (sum != S) return MSDA_ESHAPE;
-  const int tc = static_cast<int>((C * e + 15) / 16);
-  plan->threads = tc <= 256 ? 256 : (tc + 63) / 64 * 64;
-  plan->lanes = plan->threads / tc;
-  // lanes that join the sums of one group
-  int w = 1;
-  while (w < 64 && w * 2 * G <= plan->threads) w *= 2;
-  plan->team_width = w;
-  // Rows of a chunk: about 2048 workgroups in the call (8 a CU), at most 128 chunks in a level
-  // (every workgroup of the second launch reads all partial sums of its level), and at least four
-  // rows a thread.
+  const int vecs = static_cast<int>((C * e + 15) / 16);
+  plan->lanes = gn_lanes(vecs);
+  plan->tiles = (vecs + kGnThreads - 1) / kGnThreads;
+  plan->param_levels = param_levels;
+  plan->cells = static_cast<int64_t>(N) * L * G;
+  // Sums: about 2048 workgroups in the call (8 a CU) of at least kGnRowsAhead rows a thread.
+  // Writes: the rows that a thread has in flight (twice or four times as many: 165 -> 167, 179 us
+  // for the gradient of 344064 rows of 256 fp32 columns).
+  const int64_t step = static_cast<int64_t>(kGnRowsAhead) * plan->lanes;
   auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
-  int64_t r = up(static_cast<int64_t>(N) * S, 2048);
-  if (r < up(longest, 128)) r = up(longest, 128);
-  r = up(r, 4 * plan->lanes) * 4 * plan->lanes;
-  if (r > longest) r = longest;
-  GnLevels& lv = plan->lv;
-  lv.levels = L;
-  lv.param_levels = param_levels;
-  lv.rows_per_chunk = static_cast<int>(r);
-  lv.row_start[0] = lv.chunk_start[0] = 0;
-  for (int l = 0; l < L; ++l) {
-    lv.row_start[l + 1] = lv.row_start[l] + static_cast<int>(level_rows[l]);
-    lv.chunk_start[l + 1] = lv.chunk_start[l] + static_cast<int>(up(level_rows[l], r));
-  }
-  lv.chunks = lv.chunk_start[L];
-  plan->blocks = static_cast<int64_t>(N) * lv.chunks;
-  if (plan->blocks > INT32_MAX) return MSDA_ESHAPE;
+  int64_t r = up(up(static_cast<int64_t>(N) * S, 2048), step) * step;
+  gn_cut(level_rows, L, r < longest ? r : longest, &plan->sums);
+  r = step;
+  while (static_cast<int64_t>(N) * up(S, r) > (1 << 22)) r *= 2;
+  gn_cut(level_rows, L, r < longest ? r : longest, &plan->writes);
   return MSDA_OK;
 }
 
 inline size_t gn_compute_size(int dtype) { return dtype == MSDA_F64 ? 8 : 4; }
 
+// values in the workspace: forward: sums of every chunk, and the statistics where the caller has no
+// room for them; backward: sums of every chunk per group and per channel, m1 and m2
+inline int64_t gn_workspace_values(const GnPlan& plan, int N, int C, int G, bool backward) {
+  const int64_t chunks = static_cast<int64_t>(N) * plan.sums.chunks;
+  return chunks * 2 * (G + (backward ? C : 0)) + 2 * plan.cells;
+}
+
 struct GnCall {
   const void *grad_out, *x, *weight, *bias;
   void *out, *mean, *rstd, *grad_x, *grad_weight, *grad_bias, *workspace;
-  int C, G;
+  int N, C, G;
   double eps;
   bool wide;
   hipStream_t stream;
 };
 
-template <typename T, int ACT>
+template <typename T, int ACT, int MODE>
 int gn_forward(const GnCall& a, const GnPlan& plan) {
   using ct = typename Elem<T>::compute_t;
-  const dim3 grid(static_cast<unsigned>(plan.blocks)), block(plan.threads);
+  const int chunks = a.N * plan.sums.chunks;
   ct* partial = static_cast<ct*>(a.workspace);
+  ct* mean = static_cast<ct*>(a.mean);
+  ct* rstd = static_cast<ct*>(a.rstd);
+  if (mean == nullptr) {
+    mean = partial + static_cast<int64_t>(chunks) * 2 * a.G;
+    rstd = mean + plan.cells;
+  }
   Launches run;
-  run((gn_stats_kernel<T>), grid, block, 2 * sizeof(ct) * plan.lanes * a.C, a.stream,
-      static_cast<const T*>(a.x), partial, plan.lv, a.C, a.G, plan.team_width);
-  run((gn_apply_kernel<T, ACT>), grid, block, 2 * sizeof(ct) * a.G, a.stream,
-      static_cast<const T*>(a.x), static_cast<const ct*>(partial), a.weight, a.bias,
-      static_cast<T*>(a.out), static_cast<ct*>(a.mean), static_cast<ct*>(a.rstd), plan.lv, a.C, a.G,
-      plan.team_width, static_cast<ct>(a.eps), a.wide ? 1 : 0);
+  run((gn_stats_kernel<T, MODE>), dim3(chunks), dim3(kGnThreads), 2 * sizeof(ct) * plan.lanes * a.C,
+      a.stream, static_cast<const T*>(a.x), partial, plan.sums, a.C, a.G);
+  run((gn_join_kernel<ct>), dim3(a.N * plan.sums.levels, (a.G + kGnJoinGroups - 1) / kGnJoinGroups),
+      dim3(kGnThreads), 0, a.stream,
+      static_cast<const ct*>(partial), mean, rstd, plan.sums, a.C / a.G, a.G, static_cast<ct>(a.eps));
+  run((gn_apply_kernel<T, ACT, MODE>), dim3(a.N * plan.writes.chunks, plan.tiles), dim3(kGnThreads), 0,
+      a.stream, static_cast<const T*>(a.x), static_cast<const ct*>(mean), static_cast<const ct*>(rstd),
+      a.weight, a.bias, static_cast<T*>(a.out), plan.writes, a.C, a.G, plan.param_levels,
+      a.wide ? 1 : 0);
+  return run.rc;
+}
+
+template <typename T, int ACT, int MODE>
+int gn_backward(const GnCall& a, const GnPlan& plan) {
+  using ct = typename Elem<T>::compute_t;
+  const int chunks = a.N * plan.sums.chunks;
+  ct* m1 = static_cast<ct*>(a.workspace);
+  ct* m2 = m1 + plan.cells;
+  ct* partial_g = m2 + plan.cells;
+  ct* partial_c = a.grad_weight != nullptr ? partial_g + static_cast<int64_t>(chunks) * a.G * 2 : nullptr;
+  const ct* mean = static_cast<const ct*>(a.mean);
+  const ct* rstd = static_cast<const ct*>(a.rstd);
+  Launches run;
+  run((gn_bwd_stats_kernel<T, ACT, MODE>), dim3(chunks), dim3(kGnThreads),
+      2 * sizeof(ct) * plan.lanes * a.C, a.stream, static_cast<const T*>(a.grad_out),
+      static_cast<const T*>(a.x), a.weight, a.bias, mean, rstd, partial_c, partial_g, plan.sums, a.C,
+      a.G, plan.param_levels, a.wide ? 1 : 0);
+  ColumnRuns runs{};
+  runs.outer = a.N;
+  runs.pitch = plan.sums.chunks;
+  if (plan.param_levels == 1) {
+    runs.end[0] = plan.sums.chunks;
+  } else {
+    for (int l = 0; l < plan.sums.levels; ++l) {
+      runs.begin[l] = plan.sums.chunk_start[l];
+      runs.end[l] = plan.sums.chunk_start[l + 1];
+    }
+  }
+  const int groups = a.grad_x != nullptr ? a.N * plan.sums.levels * ((a.G + 31) / 32) : 0;
+  const int columns = partial_c != nullptr ? (a.C + 15) / 16 * 2 * plan.param_levels : 0;
+  if (groups + columns > 0)
+    run((gn_bwd_join_kernel<T>), dim3(groups + columns), dim3(1024), 0, a.stream,
+        static_cast<const ct*>(partial_g), static_cast<const ct*>(partial_c), m1, m2, a.grad_weight,
+        a.grad_bias, plan.sums, runs, groups, a.C, a.G, a.wide ? 1 : 0);
+  if (a.grad_x != nullptr)
+    run((gn_bwd_apply_kernel<T, ACT, MODE>), dim3(a.N * plan.writes.chunks, plan.tiles),
+        dim3(kGnThreads), 0, a.stream, static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x),
+        a.weight, a.bias, mean, rstd, static_cast<const ct*>(m1), static_cast<const ct*>(m2),
+        static_cast<T*>(a.grad_x), plan.writes, a.C, a.G, plan.param_levels, a.wide ? 1 : 0);
   return run.rc;
 }
 
 template <typename T, int ACT>
-int gn_backward(const GnCall& a, const GnPlan& plan) {
-  using ct = typename Elem<T>::compute_t;
-  const dim3 grid(static_cast<unsigned>(plan.blocks)), block(plan.threads);
-  ct* partial_g = static_cast<ct*>(a.workspace);
-  ct* partial_c = a.grad_weight != nullptr ? partial_g + plan.blocks * a.G * 2 : nullptr;
-  Launches run;
-  run((gn_bwd_stats_kernel<T, ACT>), grid, block, 2 * sizeof(ct) * plan.lanes * a.C, a.stream,
-      static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), a.weight, a.bias,
-      static_cast<const ct*>(a.mean), static_cast<const ct*>(a.rstd), partial_c, partial_g, plan.lv,
-      a.C, a.G, plan.team_width, a.wide ? 1 : 0);
-  if (partial_c != nullptr) {
-    ColumnRuns runs{};
-    runs.outer = static_cast<int>(plan.blocks / plan.lv.chunks);
-    runs.pitch = plan.lv.chunks;
-    if (plan.lv.param_levels == 1) {
-      runs.end[0] = plan.lv.chunks;
-    } else {
-      for (int l = 0; l < plan.lv.levels; ++l) {
-        runs.begin[l] = plan.lv.chunk_start[l];
-        runs.end[l] = plan.lv.chunk_start[l + 1];
-      }
-    }
-    column_sums<T>(run, partial_c, a.grad_weight, a.grad_bias, runs, plan.lv.param_levels, a.C,
-                   a.wide, a.stream);
+int gn_act_run(const GnCall& a, const GnPlan& plan, bool backward) {
+  switch (row_mode(a.C, 16 / static_cast<int>(sizeof(T)))) {
+    case kRowEven:
+      return backward ? gn_backward<T, ACT, kRowEven>(a, plan) : gn_forward<T, ACT, kRowEven>(a, plan);
+    case kRowOdd:
+      return backward ? gn_backward<T, ACT, kRowOdd>(a, plan) : gn_forward<T, ACT, kRowOdd>(a, plan);
+    default:
+      return backward ? gn_backward<T, ACT, kRowShort>(a, plan) : gn_forward<T, ACT, kRowShort>(a, plan);
   }
-  if (a.grad_x != nullptr)
-    run((gn_bwd_apply_kernel<T, ACT>), grid, block, 2 * sizeof(ct) * a.G, a.stream,
-        static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), a.weight, a.bias,
-        static_cast<const ct*>(a.mean), static_cast<const ct*>(a.rstd),
-        static_cast<const ct*>(partial_g), static_cast<T*>(a.grad_x), plan.lv, a.C, a.G,
-        plan.team_width, a.wide ? 1 : 0);
-  return run.rc;
 }
 
 template <typename T>
 int gn_run(const GnCall& a, const GnPlan& plan, int activation, bool backward) {
   switch (activation) {
-    case kGnRelu: return backward ? gn_backward<T, kGnRelu>(a, plan) : gn_forward<T, kGnRelu>(a, plan);
-    case kGnSilu: return backward ? gn_backward<T, kGnSilu>(a, plan) : gn_forward<T, kGnSilu>(a, plan);
-    case kGnGelu: return backward ? gn_backward<T, kGnGelu>(a, plan) : gn_forward<T, kGnGelu>(a, plan);
-    default: return backward ? gn_backward<T, kGnNone>(a, plan) : gn_forward<T, kGnNone>(a, plan);
+    case kGnRelu: return gn_act_run<T, kGnRelu>(a, plan, backward);
+    case kGnSilu: return gn_act_run<T, kGnSilu>(a, plan, backward);
+    case kGnGelu: return gn_act_run<T, kGnGelu>(a, plan, backward);
+    default: return gn_act_run<T, kGnNone>(a, plan, backward);
   }
 }
 
@@ -392,6 +458,7 @@ int msda_dropout_add_norm_forward(const void* x, const void* residual, const voi
   a.rng_state = rng_state;
   a.rows = rows;
   a.C = C;
+  a.dtype_res = dtype_residual;
   a.site = static_cast<uint32_t>(site);
   a.eps = eps;
   a.wide = dtype_param != MSDA_BF16 && dtype_param != MSDA_F16;
@@ -403,7 +470,9 @@ size_t msda_dropout_add_norm_workspace_bytes(int64_t rows, int C, int dtype_x, i
   using namespace msda;
   DropArgs d;
   if (add_norm_check(rows, C, 0.0, 0, dtype_x, dtype_residual, dtype_residual, &d) != MSDA_OK) return 0;
-  return static_cast<size_t>(add_norm_bwd_blocks(rows)) * 2 * C * (dtype_residual == MSDA_F64 ? 8 : 4);
+  const int64_t blocks = add_norm_bwd_grid(rows, C, dtype_residual).blocks;
+  return static_cast<size_t>(blocks + (blocks > kColumnSplit ? kColumnSegments : 0)) * 2 * C *
+         (dtype_residual == MSDA_F64 ? 8 : 4);
 }
 
 int msda_dropout_add_norm_backward(const void* grad_out, const void* x, const void* residual,
@@ -444,6 +513,7 @@ int msda_dropout_add_norm_backward(const void* grad_out, const void* x, const vo
   a.rng_state = rng_state;
   a.rows = rows;
   a.C = C;
+  a.dtype_res = dtype_residual;
   a.site = static_cast<uint32_t>(site);
   a.wide = dtype_param != MSDA_BF16 && dtype_param != MSDA_F16;
   a.stream = static_cast<hipStream_t>(hip_stream);
@@ -457,7 +527,7 @@ size_t msda_group_norm_workspace_bytes(const int64_t* level_rows_host, int N, in
   if (level_rows_host == nullptr ||
       gn_plan(level_rows_host, N, S, C, G, L, 1, kGnNone, dtype, dtype, &plan) != MSDA_OK)
     return 0;
-  return static_cast<size_t>(plan.blocks) * 2 * (G + (backward ? C : 0)) * gn_compute_size(dtype);
+  return static_cast<size_t>(gn_workspace_values(plan, N, C, G, backward != 0)) * gn_compute_size(dtype);
 }
 
 int msda_group_norm_forward(const void* x, const void* weight, const void* bias, void* out,
@@ -487,6 +557,7 @@ int msda_group_norm_forward(const void* x, const void* weight, const void* bias,
   a.mean = mean;
   a.rstd = rstd;
   a.workspace = workspace;
+  a.N = N;
   a.C = C;
   a.G = G;
   a.eps = eps;
@@ -527,6 +598,7 @@ int msda_group_norm_backward(const void* grad_out, const void* x, const void* we
   a.grad_weight = grad_weight;
   a.grad_bias = grad_bias;
   a.workspace = workspace;
+  a.N = N;
   a.C = C;
   a.G = G;
   a.wide = dtype_param != MSDA_BF16 && dtype_param != MSDA_F16;

@@ -6,11 +6,11 @@
 //   with dz = dy * act'(z):  db = sum dz,  dw = sum dz * u  (over samples and rows),
 //   dx = s * (w dz - m1 - u * m2),  m1 = mean (w dz),  m2 = mean (w dz u)  (over rows and group)
 //
-// A level's rows are cut into chunks, a workgroup each.  Threads lie along the channels (16 bytes a
-// thread) and then along the rows, so a thread keeps its channels for the whole chunk and sums per
-// channel in registers; groups are formed from channels once per chunk.  Two launches a direction:
-// the first leaves partial sums per chunk, every workgroup of the second joins the partial sums of
-// its level (the same numbers in the same order everywhere) and writes its chunk.
+// Three launches a direction: sums per chunk of rows, a join of the chunks' sums per level, and the
+// pass that writes.  Threads lie along the channels (16 bytes a thread) and then along the rows, so a
+// thread keeps its channels for the whole chunk and sums per channel in registers; groups are formed
+// from channels once per chunk.  The passes that write take short chunks (a workgroup a few rows a
+// thread, all their loads in flight at once), which need the level's joined sums and not its chunks'.
 #pragma once
 
 #include "msda_vec.h"
@@ -19,33 +19,60 @@ namespace msda {
 
 enum GnAct { kGnNone = 0, kGnRelu = 1, kGnSilu = 2, kGnGelu = 3 };
 
-struct GnLevels {
-  int levels, chunks, rows_per_chunk, param_levels;
+constexpr int kGnThreads = 256;
+constexpr int kGnRowsAhead = 4;  // rows of a thread whose loads are in flight together
+
+// The rows of every sample cut into levels and the levels into chunks.
+struct GnCut {
+  int levels, chunks, rows_per_chunk;
   int row_start[kMaxNormLevels + 1];
   int chunk_start[kMaxNormLevels + 1];
 };
 
 struct GnChunk {
   int level, rows;
+  int n;
   int64_t first_row;  // within the tensor
-  int64_t n;
 };
 
-__device__ __forceinline__ GnChunk gn_chunk(const GnLevels& lv, int block) {
+__device__ __forceinline__ GnChunk gn_chunk(const GnCut& cut, int block) {
   GnChunk c;
-  c.n = block / lv.chunks;
-  const int chunk = block - static_cast<int>(c.n) * lv.chunks;
+  c.n = block / cut.chunks;
+  const int chunk = block - c.n * cut.chunks;
   c.level = 0;
-  while (c.level + 1 < lv.levels && chunk >= lv.chunk_start[c.level + 1]) ++c.level;
-  const int row = lv.row_start[c.level] + (chunk - lv.chunk_start[c.level]) * lv.rows_per_chunk;
-  c.rows = min(lv.rows_per_chunk, lv.row_start[c.level + 1] - row);
-  c.first_row = c.n * lv.row_start[lv.levels] + row;
+  while (c.level + 1 < cut.levels && chunk >= cut.chunk_start[c.level + 1]) ++c.level;
+  const int row = cut.row_start[c.level] + (chunk - cut.chunk_start[c.level]) * cut.rows_per_chunk;
+  c.rows = min(cut.rows_per_chunk, cut.row_start[c.level + 1] - row);
+  c.first_row = static_cast<int64_t>(c.n) * cut.row_start[cut.levels] + row;
   return c;
 }
+
+// row lanes of a workgroup for rows of `vecs` vectors
+__host__ __device__ inline int gn_lanes(int vecs) { return vecs < kGnThreads ? kGnThreads / vecs : 1; }
 
 // rows of a chunk of `rows` that row lane r of `lanes` handles
 __device__ __forceinline__ int gn_lane_rows(int rows, int r, int lanes) {
   return r < rows ? (rows - r + lanes - 1) / lanes : 0;
+}
+
+// Calls f(Pack (&)[K], rows r0, r0 + lanes, ...) for the thread's rows with the loads of
+// kGnRowsAhead rows issued before the first is used.  `load` fills one row's packs.
+template <typename P, typename Load, typename Use>
+__device__ __forceinline__ void gn_rows(int r0, int rows, int lanes, Load load, Use use) {
+  constexpr int U = kGnRowsAhead;
+  int r = r0;
+  for (; r + (U - 1) * lanes < rows; r += U * lanes) {
+    P p[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) load(p[k], r + k * lanes);
+#pragma unroll
+    for (int k = 0; k < U; ++k) use(p[k], r + k * lanes);
+  }
+  for (; r < rows; r += lanes) {
+    P p;
+    load(p, r);
+    use(p, r);
+  }
 }
 
 // (count, mean, M2) of a union of two sets (T. F. Chan, G. H. Golub, R. J. LeVeque 1979)
@@ -76,9 +103,39 @@ __device__ __forceinline__ void team_moments(Moments<CT>& m, int width) {
     m = a;
   }
 }
+template <typename CT>
+__device__ __forceinline__ void team_add2(CT& a, CT& b, int width) {
+  for (int off = 1; off < width; off <<= 1) {
+    a += __shfl_xor(a, off, 64);
+    b += __shfl_xor(b, off, 64);
+  }
+}
+
+// lanes that join the sums of one group in a workgroup of `threads`
+__host__ __device__ inline int gn_team_width(int threads, int G) {
+  int w = 1;
+  while (w < 64 && w * 2 * G <= threads) w *= 2;
+  return w;
+}
+
+// the VE values of `src` (one a group) that belong to the columns of a span
+template <int VE, int MODE, typename CT>
+__device__ __forceinline__ void gn_spread(const CT* __restrict__ src, const Span<VE, MODE>& sp, int cpg,
+                                          CT* v) {
+  int g = sp.c / cpg, at = sp.c - g * cpg;
+#pragma unroll
+  for (int i = 0; i < VE; ++i) {
+    v[i] = i < sp.count ? src[g] : CT(0);
+    if (++at == cpg) {
+      at = 0;
+      ++g;
+    }
+  }
+}
 
 // ---- activation -----------------------------------------------------------------------------------
-__device__ __forceinline__ float gn_sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+// (v_rcp_f32 is within one step of 1 / x: a division would cost ten instructions more an element)
+__device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 __device__ __forceinline__ double gn_sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
 template <int ACT, typename CT>
@@ -104,67 +161,68 @@ __device__ __forceinline__ CT gn_slope(CT z) {
 }
 
 // ---- forward ----------------------------------------------------------------------------------------
-// partial[(n * chunks + chunk) * G + g] = (mean, M2) of the chunk's rows of group g.
-// Thread-level sums are taken about the first value that the thread reads of each channel: at most
-// rows_per_chunk additions each, so an outlying first value costs at most that many roundings of
-// what it adds to the variance itself.
+// partial[(block * G + g) * 2] = (mean, M2) of the chunk's rows of group g.
+// Thread-level sums are taken about the first value that the thread reads of each channel, so a
+// common offset of the values costs nothing; an outlying first value costs at most a rounding per
+// row of what it adds to the variance itself.
 // Dynamic LDS: 2 * row lanes * C values.
-template <typename T>
-__global__ __launch_bounds__(1024) void gn_stats_kernel(
-    const T* __restrict__ x, typename Elem<T>::compute_t* __restrict__ partial, GnLevels lv, int C,
-    int G, int team_width) {
+template <typename T, int MODE>
+__global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(
+    const T* __restrict__ x, typename Elem<T>::compute_t* __restrict__ partial, GnCut cut, int C,
+    int G) {
   using ct = typename Elem<T>::compute_t;
   constexpr int VE = 16 / sizeof(T);
+  using P = Pack<T, VE>;
   extern __shared__ __align__(16) char gn_lds[];
-  const int tc = (C + VE - 1) / VE, lanes = blockDim.x / tc;
+  const int vecs = (C + VE - 1) / VE, lanes = gn_lanes(vecs);
   ct* lds_mean = reinterpret_cast<ct*>(gn_lds);
   ct* lds_m2 = lds_mean + lanes * C;
-  const GnChunk ch = gn_chunk(lv, blockIdx.x);
-  const int r0 = threadIdx.x / tc, c0 = (threadIdx.x - r0 * tc) * VE;
-  const int count = min(VE, C - c0);
-  if (r0 < lanes) {
-    const T* src = x + ch.first_row * C + c0;
+  const GnChunk ch = gn_chunk(cut, blockIdx.x);
+  const T* src = x + ch.first_row * C;
+  const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
+  for (int k = threadIdx.x - r0 * vecs; k < vecs && r0 < lanes; k += kGnThreads) {
+    const auto sp = Span<VE, MODE>::at(k, C);
     ct pivot[VE], s[VE], q[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) pivot[i] = s[i] = q[i] = 0;
     if (r0 < ch.rows) {
-      Pack<T, VE> p;
-      p.load(src + static_cast<int64_t>(r0) * C, count);
+      P p;
+      sp.load(p, src + static_cast<int64_t>(r0) * C);
       p.unpack(pivot);
     }
-#pragma unroll 4
-    for (int r = r0 + lanes; r < ch.rows; r += lanes) {
-      Pack<T, VE> p;
-      p.load(src + static_cast<int64_t>(r) * C, count);
-      ct v[VE];
-      p.unpack(v);
+    gn_rows<P>(
+        r0 + lanes, ch.rows, lanes,
+        [&](P& p, int r) { sp.load(p, src + static_cast<int64_t>(r) * C); },
+        [&](P& p, int) {
+          ct v[VE];
+          p.unpack(v);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const ct d = v[i] - pivot[i];
-        s[i] += d;
-        q[i] += d * d;
-      }
-    }
+          for (int i = 0; i < VE; ++i) {
+            const ct d = v[i] - pivot[i];
+            s[i] += d;
+            q[i] += d * d;
+          }
+        });
     const int n = gn_lane_rows(ch.rows, r0, lanes);
     const ct inv = n > 0 ? ct(1) / static_cast<ct>(n) : ct(0);
 #pragma unroll
     for (int i = 0; i < VE; ++i)
-      if (i < count) {
-        lds_mean[r0 * C + c0 + i] = pivot[i] + s[i] * inv;
+      if (sp.owns(i)) {
         const ct m2 = q[i] - s[i] * s[i] * inv;
-        lds_m2[r0 * C + c0 + i] = m2 < ct(0) ? ct(0) : m2;  // (NaN stays)
+        lds_mean[r0 * C + sp.c + i] = pivot[i] + s[i] * inv;
+        lds_m2[r0 * C + sp.c + i] = m2 < ct(0) ? ct(0) : m2;  // (NaN stays)
       }
   }
   __syncthreads();
-  const int cpg = C / G, teams = blockDim.x / team_width;
-  const int j = threadIdx.x & (team_width - 1);
-  for (int g = threadIdx.x / team_width; g < G; g += teams) {
+  const int cpg = C / G, width = gn_team_width(kGnThreads, G), teams = kGnThreads / width;
+  const int j = threadIdx.x & (width - 1);
+  for (int g = threadIdx.x / width; g < G; g += teams) {
     Moments<ct> m{0, 0, 0};
-    for (int e = j; e < lanes * cpg; e += team_width) {
+    for (int e = j; e < lanes * cpg; e += width) {
       const int r = e / cpg, at = r * C + g * cpg + (e - r * cpg);
       m.add(static_cast<ct>(gn_lane_rows(ch.rows, r, lanes)), lds_mean[at], lds_m2[at]);
     }
-    team_moments(m, team_width);
+    team_moments(m, width);
     if (j == 0) {
       ct* dst = partial + (static_cast<int64_t>(blockIdx.x) * G + g) * 2;
       dst[0] = m.mean;
@@ -173,147 +231,157 @@ __global__ __launch_bounds__(1024) void gn_stats_kernel(
   }
 }
 
-// mean and M2 of every group of the block's level, from the chunks' partial sums
+// mean and rstd (N, levels, G) from the chunks' sums: the mean of the means, then M2 about it
+// (sum of the chunks' M2 and of n_k (mean_k - mean)^2; the second reading comes from the cache).
+// blockIdx.x: (sample, level), blockIdx.y: tile of kGnJoinGroups groups.
+constexpr int kGnJoinGroups = 8;
 template <typename CT>
-__device__ __forceinline__ void gn_join_stats(const CT* __restrict__ partial, const GnLevels& lv,
-                                              const GnChunk& ch, int cpg, int G, int team_width,
-                                              CT eps, CT* lds_mean, CT* lds_rstd) {
-  const int begin = lv.chunk_start[ch.level], end = lv.chunk_start[ch.level + 1];
-  const int rows = lv.row_start[ch.level + 1] - lv.row_start[ch.level];
-  const int teams = blockDim.x / team_width, j = threadIdx.x & (team_width - 1);
-  for (int g = threadIdx.x / team_width; g < G; g += teams) {
-    Moments<CT> m{0, 0, 0};
-    for (int k = begin + j; k < end; k += team_width) {
-      const CT* src = partial + ((ch.n * lv.chunks + k) * G + g) * 2;
-      const int in = min(lv.rows_per_chunk, rows - (k - begin) * lv.rows_per_chunk);
-      m.add(static_cast<CT>(in) * static_cast<CT>(cpg), src[0], src[1]);
-    }
-    team_moments(m, team_width);
-    if (j == 0) {
-      lds_mean[g] = m.mean;
-      lds_rstd[g] = CT(1) / sqrt(m.m2 / (static_cast<CT>(rows) * static_cast<CT>(cpg)) + eps);
-    }
+__global__ __launch_bounds__(kGnThreads) void gn_join_kernel(const CT* __restrict__ partial,
+                                                             CT* __restrict__ mean,
+                                                             CT* __restrict__ rstd, GnCut cut, int cpg,
+                                                             int G, CT eps) {
+  constexpr int WIDTH = kGnThreads / kGnJoinGroups;
+  const int n = blockIdx.x / cut.levels, level = blockIdx.x - n * cut.levels;
+  const int chunks = cut.chunk_start[level + 1] - cut.chunk_start[level];
+  const int rows = cut.row_start[level + 1] - cut.row_start[level];
+  const int j = threadIdx.x % WIDTH, g = blockIdx.y * kGnJoinGroups + threadIdx.x / WIDTH;
+  if (g >= G) return;
+  const CT* src =
+      partial + ((static_cast<int64_t>(n) * cut.chunks + cut.chunk_start[level]) * G + g) * 2;
+  const CT share = CT(1) / static_cast<CT>(rows);
+  auto chunk_rows = [&](int k) {
+    return static_cast<CT>(min(cut.rows_per_chunk, rows - k * cut.rows_per_chunk));
+  };
+  // about the first chunk's mean, so that a common offset costs nothing
+  const CT pivot = src[0];
+  CT mu = 0;
+#pragma unroll 4
+  for (int k = j; k < chunks; k += WIDTH)
+    mu += chunk_rows(k) * share * (src[static_cast<int64_t>(k) * G * 2] - pivot);
+  for (int off = 1; off < WIDTH; off <<= 1) mu += __shfl_xor(mu, off, 64);
+  CT m2 = 0;
+#pragma unroll 4
+  for (int k = j; k < chunks; k += WIDTH) {
+    const CT* at = src + static_cast<int64_t>(k) * G * 2;
+    const CT d = at[0] - pivot - mu;
+    m2 += at[1] + chunk_rows(k) * static_cast<CT>(cpg) * d * d;
+  }
+  for (int off = 1; off < WIDTH; off <<= 1) m2 += __shfl_xor(m2, off, 64);
+  if (j == 0) {
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * G + g;
+    mean[at] = pivot + mu;
+    rstd[at] = CT(1) / sqrt(m2 / (static_cast<CT>(rows) * static_cast<CT>(cpg)) + eps);
   }
 }
 
-// mean and rstd (N, levels, G) may be NULL (no gradient wanted).  Dynamic LDS: 2 G values.
-template <typename T, int ACT>
-__global__ __launch_bounds__(1024) void gn_apply_kernel(
-    const T* __restrict__ x, const typename Elem<T>::compute_t* __restrict__ partial,
-    const void* __restrict__ weight, const void* __restrict__ bias, T* __restrict__ out,
-    typename Elem<T>::compute_t* __restrict__ mean, typename Elem<T>::compute_t* __restrict__ rstd,
-    GnLevels lv, int C, int G, int team_width, typename Elem<T>::compute_t eps, int wide) {
+// blockIdx.y: tile of kGnThreads vectors of a row
+template <typename T, int ACT, int MODE>
+__global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(
+    const T* __restrict__ x, const typename Elem<T>::compute_t* __restrict__ mean,
+    const typename Elem<T>::compute_t* __restrict__ rstd, const void* __restrict__ weight,
+    const void* __restrict__ bias, T* __restrict__ out, GnCut cut, int C, int G, int param_levels,
+    int wide) {
   using ct = typename Elem<T>::compute_t;
   constexpr int VE = 16 / sizeof(T);
-  extern __shared__ __align__(16) char gn_lds[];
-  ct* lds_mean = reinterpret_cast<ct*>(gn_lds);
-  ct* lds_rstd = lds_mean + G;
-  const GnChunk ch = gn_chunk(lv, blockIdx.x);
-  const int cpg = C / G;
-  gn_join_stats(partial, lv, ch, cpg, G, team_width, eps, lds_mean, lds_rstd);
-  __syncthreads();
-  const int chunk = blockIdx.x % lv.chunks;
-  if (mean != nullptr && chunk == lv.chunk_start[ch.level]) {
-    for (int g = threadIdx.x; g < G; g += blockDim.x) {
-      const int64_t at = (ch.n * lv.levels + ch.level) * G + g;
-      mean[at] = lds_mean[g];
-      rstd[at] = lds_rstd[g];
-    }
-  }
-  const int tc = (C + VE - 1) / VE, lanes = blockDim.x / tc;
-  const int r0 = threadIdx.x / tc, c0 = (threadIdx.x - r0 * tc) * VE;
-  if (r0 >= lanes) return;
-  const int count = min(VE, C - c0);
-  const int64_t pl = lv.param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
-  ct mu[VE], a[VE], b[VE];
+  using P = Pack<T, VE>;
+  const int vecs = (C + VE - 1) / VE, lanes = gn_lanes(vecs), cpg = C / G;
+  const GnChunk ch = gn_chunk(cut, blockIdx.x);
+  const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
+  const int k = threadIdx.x - r0 * vecs + blockIdx.y * kGnThreads;
+  if (r0 >= lanes || k >= vecs) return;
+  const auto sp = Span<VE, MODE>::at(k, C);
+  const int64_t pl = param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
+  const int64_t sg = (static_cast<int64_t>(ch.n) * cut.levels + ch.level) * G;
+  ct mu[VE], a[VE], b[VE], w[VE];
+  gn_spread(mean + sg, sp, cpg, mu);
+  gn_spread(rstd + sg, sp, cpg, a);
+  load_params<T>(weight, pl, sp, wide != 0, w);
+  load_params<T>(bias, pl, sp, wide != 0, b);
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    mu[i] = a[i] = b[i] = 0;
-    if (i < count) {
-      const int g = (c0 + i) / cpg;
-      mu[i] = lds_mean[g];
-      a[i] = lds_rstd[g] * load_param<T>(weight, pl + c0 + i, wide != 0);
-      b[i] = load_param<T>(bias, pl + c0 + i, wide != 0);
-    }
-  }
-  const int64_t base = ch.first_row * C + c0;
-#pragma unroll 4
-  for (int r = r0; r < ch.rows; r += lanes) {
-    Pack<T, VE> p;
-    p.load(x + base + static_cast<int64_t>(r) * C, count);
-    ct v[VE];
-    p.unpack(v);
+  for (int i = 0; i < VE; ++i) a[i] *= w[i];
+  const T* src = x + ch.first_row * C;
+  T* dst = out + ch.first_row * C;
+  gn_rows<P>(
+      r0, ch.rows, lanes, [&](P& p, int r) { sp.load(p, src + static_cast<int64_t>(r) * C); },
+      [&](P& p, int r) {
+        ct v[VE];
+        p.unpack(v);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) v[i] = gn_act<ACT>((v[i] - mu[i]) * a[i] + b[i]);
-    p.pack(v);
-    p.store(out + base + static_cast<int64_t>(r) * C, count);
-  }
+        for (int i = 0; i < VE; ++i) v[i] = gn_act<ACT>((v[i] - mu[i]) * a[i] + b[i]);
+        p.pack(v);
+        sp.store(p, dst + static_cast<int64_t>(r) * C);
+      });
 }
 
 // ---- gradient ---------------------------------------------------------------------------------------
+template <typename T, int VE>
+struct GnPair {
+  Pack<T, VE> x, g;
+};
+
 // Per chunk: partial_c[(block * 2 + k) * C + c] = sum over rows of dz * u (k = 0) and dz (k = 1), for
 // the parameters; partial_g[(block * G + g) * 2 + k] = sum over the group of w dz (k = 0) and
 // w dz u (k = 1), for dx.  partial_c may be NULL.  Dynamic LDS: 2 * row lanes * C values.
-template <typename T, int ACT>
-__global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(
+template <typename T, int ACT, int MODE>
+__global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(
     const T* __restrict__ grad_out, const T* __restrict__ x, const void* __restrict__ weight,
     const void* __restrict__ bias, const typename Elem<T>::compute_t* __restrict__ mean,
     const typename Elem<T>::compute_t* __restrict__ rstd,
     typename Elem<T>::compute_t* __restrict__ partial_c,
-    typename Elem<T>::compute_t* __restrict__ partial_g, GnLevels lv, int C, int G, int team_width,
+    typename Elem<T>::compute_t* __restrict__ partial_g, GnCut cut, int C, int G, int param_levels,
     int wide) {
   using ct = typename Elem<T>::compute_t;
   constexpr int VE = 16 / sizeof(T);
+  using P = GnPair<T, VE>;
   extern __shared__ __align__(16) char gn_lds[];
-  const int tc = (C + VE - 1) / VE, lanes = blockDim.x / tc;
+  const int vecs = (C + VE - 1) / VE, lanes = gn_lanes(vecs), cpg = C / G;
   ct* lds_dw = reinterpret_cast<ct*>(gn_lds);
   ct* lds_db = lds_dw + lanes * C;
-  const GnChunk ch = gn_chunk(lv, blockIdx.x);
-  const int r0 = threadIdx.x / tc, c0 = (threadIdx.x - r0 * tc) * VE;
-  const int count = min(VE, C - c0), cpg = C / G;
-  const int64_t pl = lv.param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
-  const int64_t sg = (ch.n * lv.levels + ch.level) * G;
-  if (r0 < lanes) {
+  const GnChunk ch = gn_chunk(cut, blockIdx.x);
+  const int64_t pl = param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
+  const int64_t sg = (static_cast<int64_t>(ch.n) * cut.levels + ch.level) * G;
+  const T* sx = x + ch.first_row * C;
+  const T* sd = grad_out + ch.first_row * C;
+  const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
+  for (int k = threadIdx.x - r0 * vecs; k < vecs && r0 < lanes; k += kGnThreads) {
+    const auto sp = Span<VE, MODE>::at(k, C);
     ct mu[VE], s[VE], w[VE], b[VE], dw[VE], db[VE];
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      mu[i] = s[i] = w[i] = b[i] = dw[i] = db[i] = 0;
-      if (i < count) {
-        const int g = (c0 + i) / cpg;
-        mu[i] = mean[sg + g];
-        s[i] = rstd[sg + g];
-        if (ACT != kGnNone) {
-          w[i] = load_param<T>(weight, pl + c0 + i, wide != 0);
-          b[i] = load_param<T>(bias, pl + c0 + i, wide != 0);
-        }
-      }
+    gn_spread(mean + sg, sp, cpg, mu);
+    gn_spread(rstd + sg, sp, cpg, s);
+    if constexpr (ACT != kGnNone) {
+      load_params<T>(weight, pl, sp, wide != 0, w);
+      load_params<T>(bias, pl, sp, wide != 0, b);
     }
-    const int64_t base = ch.first_row * C + c0;
-#pragma unroll 4
-    for (int r = r0; r < ch.rows; r += lanes) {
-      Pack<T, VE> px, pg;
-      px.load(x + base + static_cast<int64_t>(r) * C, count);
-      pg.load(grad_out + base + static_cast<int64_t>(r) * C, count);
-      ct xv[VE], gv[VE];
-      px.unpack(xv);
-      pg.unpack(gv);
 #pragma unroll
-      for (int i = 0; i < VE; ++i) {
-        const ct u = (xv[i] - mu[i]) * s[i];
-        const ct dz = ACT == kGnNone ? gv[i] : gv[i] * gn_slope<ACT>(u * w[i] + b[i]);
-        dw[i] += dz * u;
-        db[i] += dz;
-      }
-    }
+    for (int i = 0; i < VE; ++i) dw[i] = db[i] = 0;
+    gn_rows<P>(
+        r0, ch.rows, lanes,
+        [&](P& p, int r) {
+          sp.load(p.x, sx + static_cast<int64_t>(r) * C);
+          sp.load(p.g, sd + static_cast<int64_t>(r) * C);
+        },
+        [&](P& p, int) {
+          ct xv[VE], gv[VE];
+          p.x.unpack(xv);
+          p.g.unpack(gv);
+#pragma unroll
+          for (int i = 0; i < VE; ++i) {
+            const ct u = (xv[i] - mu[i]) * s[i];
+            ct dz = gv[i];
+            if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[i] + b[i]);
+            dw[i] += dz * u;
+            db[i] += dz;
+          }
+        });
 #pragma unroll
     for (int i = 0; i < VE; ++i)
-      if (i < count) {
-        lds_dw[r0 * C + c0 + i] = dw[i];
-        lds_db[r0 * C + c0 + i] = db[i];
+      if (sp.owns(i)) {
+        lds_dw[r0 * C + sp.c + i] = dw[i];
+        lds_db[r0 * C + sp.c + i] = db[i];
       }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < C; c += blockDim.x) {
+  for (int c = threadIdx.x; c < C; c += kGnThreads) {
     ct dw = 0, db = 0;
     for (int r = 0; r < lanes; ++r) {
       dw += lds_dw[r * C + c];
@@ -329,17 +397,15 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(
     lds_db[c] = db * w;
   }
   __syncthreads();
-  const int teams = blockDim.x / team_width, j = threadIdx.x & (team_width - 1);
-  for (int g = threadIdx.x / team_width; g < G; g += teams) {
+  const int width = gn_team_width(kGnThreads, G), teams = kGnThreads / width;
+  const int j = threadIdx.x & (width - 1);
+  for (int g = threadIdx.x / width; g < G; g += teams) {
     ct m1 = 0, m2 = 0;
-    for (int e = j; e < cpg; e += team_width) {
+    for (int e = j; e < cpg; e += width) {
       m1 += lds_db[g * cpg + e];
       m2 += lds_dw[g * cpg + e];
     }
-    for (int off = 1; off < team_width; off <<= 1) {
-      m1 += __shfl_xor(m1, off, 64);
-      m2 += __shfl_xor(m2, off, 64);
-    }
+    team_add2(m1, m2, width);
     if (j == 0) {
       ct* dst = partial_g + (static_cast<int64_t>(blockIdx.x) * G + g) * 2;
       dst[0] = m1;
@@ -348,79 +414,93 @@ __global__ __launch_bounds__(1024) void gn_bwd_stats_kernel(
   }
 }
 
-// Dynamic LDS: 2 G values.
-template <typename T, int ACT>
-__global__ __launch_bounds__(1024) void gn_bwd_apply_kernel(
+// Joins what the chunks left, in one launch: the first `groups` workgroups (one a (sample, level) and
+// tile of 32 groups) write m1 and m2 (N, levels, G), the others the parameters' gradients.
+template <typename T>
+__global__ __launch_bounds__(1024) void gn_bwd_join_kernel(
+    const typename Elem<T>::compute_t* __restrict__ partial_g,
+    const typename Elem<T>::compute_t* __restrict__ partial_c,
+    typename Elem<T>::compute_t* __restrict__ m1, typename Elem<T>::compute_t* __restrict__ m2,
+    void* __restrict__ grad_weight, void* __restrict__ grad_bias, GnCut cut, ColumnRuns runs, int groups,
+    int C, int G, int wide) {
+  using ct = typename Elem<T>::compute_t;
+  if (static_cast<int>(blockIdx.x) >= groups) {
+    const int tiles = (C + 15) / 16, b = blockIdx.x - groups;
+    column_sums<T>(partial_c, grad_weight, grad_bias, runs, C, wide != 0, b % tiles,
+                   (b / tiles) & 1, b / tiles / 2);
+    return;
+  }
+  const int tiles = (G + 31) / 32, cell = blockIdx.x / tiles;
+  const int n = cell / cut.levels, level = cell - n * cut.levels;
+  const int chunks = cut.chunk_start[level + 1] - cut.chunk_start[level];
+  const int rows = cut.row_start[level + 1] - cut.row_start[level];
+  const ct inv = ct(1) / (static_cast<ct>(rows) * static_cast<ct>(C / G));
+  const int j = threadIdx.x & 31, g = (blockIdx.x - cell * tiles) * 32 + (threadIdx.x >> 5);
+  if (g >= G) return;
+  const ct* src =
+      partial_g + ((static_cast<int64_t>(n) * cut.chunks + cut.chunk_start[level]) * G + g) * 2;
+  ct a = 0, b = 0;
+#pragma unroll 4
+  for (int k = j; k < chunks; k += 32) {
+    a += src[static_cast<int64_t>(k) * G * 2];
+    b += src[static_cast<int64_t>(k) * G * 2 + 1];
+  }
+  team_add2(a, b, 32);
+  if (j == 0) {
+    m1[static_cast<int64_t>(cell) * G + g] = a * inv;
+    m2[static_cast<int64_t>(cell) * G + g] = b * inv;
+  }
+}
+
+template <typename T, int ACT, int MODE>
+__global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(
     const T* __restrict__ grad_out, const T* __restrict__ x, const void* __restrict__ weight,
     const void* __restrict__ bias, const typename Elem<T>::compute_t* __restrict__ mean,
     const typename Elem<T>::compute_t* __restrict__ rstd,
-    const typename Elem<T>::compute_t* __restrict__ partial_g, T* __restrict__ grad_x, GnLevels lv,
-    int C, int G, int team_width, int wide) {
+    const typename Elem<T>::compute_t* __restrict__ m1,
+    const typename Elem<T>::compute_t* __restrict__ m2, T* __restrict__ grad_x, GnCut cut, int C, int G,
+    int param_levels, int wide) {
   using ct = typename Elem<T>::compute_t;
   constexpr int VE = 16 / sizeof(T);
-  extern __shared__ __align__(16) char gn_lds[];
-  ct* lds_m1 = reinterpret_cast<ct*>(gn_lds);
-  ct* lds_m2 = lds_m1 + G;
-  const GnChunk ch = gn_chunk(lv, blockIdx.x);
-  const int cpg = C / G;
-  const int teams = blockDim.x / team_width, j = threadIdx.x & (team_width - 1);
-  const int rows = lv.row_start[ch.level + 1] - lv.row_start[ch.level];
-  const ct inv = ct(1) / (static_cast<ct>(rows) * static_cast<ct>(cpg));
-  for (int g = threadIdx.x / team_width; g < G; g += teams) {
-    ct m1 = 0, m2 = 0;
-    for (int k = lv.chunk_start[ch.level] + j; k < lv.chunk_start[ch.level + 1]; k += team_width) {
-      const ct* src = partial_g + ((ch.n * lv.chunks + k) * G + g) * 2;
-      m1 += src[0];
-      m2 += src[1];
-    }
-    for (int off = 1; off < team_width; off <<= 1) {
-      m1 += __shfl_xor(m1, off, 64);
-      m2 += __shfl_xor(m2, off, 64);
-    }
-    if (j == 0) {
-      lds_m1[g] = m1 * inv;
-      lds_m2[g] = m2 * inv;
-    }
-  }
-  __syncthreads();
-  const int tc = (C + VE - 1) / VE, lanes = blockDim.x / tc;
-  const int r0 = threadIdx.x / tc, c0 = (threadIdx.x - r0 * tc) * VE;
-  if (r0 >= lanes) return;
-  const int count = min(VE, C - c0);
-  const int64_t pl = lv.param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
-  const int64_t sg = (ch.n * lv.levels + ch.level) * G;
-  ct mu[VE], s[VE], w[VE], b[VE], m1[VE], m2[VE];
+  using P = GnPair<T, VE>;
+  const int vecs = (C + VE - 1) / VE, lanes = gn_lanes(vecs), cpg = C / G;
+  const GnChunk ch = gn_chunk(cut, blockIdx.x);
+  const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
+  const int k = threadIdx.x - r0 * vecs + blockIdx.y * kGnThreads;
+  if (r0 >= lanes || k >= vecs) return;
+  const auto sp = Span<VE, MODE>::at(k, C);
+  const int64_t pl = param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
+  const int64_t sg = (static_cast<int64_t>(ch.n) * cut.levels + ch.level) * G;
+  ct mu[VE], s[VE], w[VE], b[VE], a1[VE], a2[VE];
+  gn_spread(mean + sg, sp, cpg, mu);
+  gn_spread(rstd + sg, sp, cpg, s);
+  gn_spread(m1 + sg, sp, cpg, a1);
+  gn_spread(m2 + sg, sp, cpg, a2);
+  load_params<T>(weight, pl, sp, wide != 0, w);
+  if constexpr (ACT != kGnNone) load_params<T>(bias, pl, sp, wide != 0, b);
+  const T* sx = x + ch.first_row * C;
+  const T* sd = grad_out + ch.first_row * C;
+  T* dst = grad_x + ch.first_row * C;
+  gn_rows<P>(
+      r0, ch.rows, lanes,
+      [&](P& p, int r) {
+        sp.load(p.x, sx + static_cast<int64_t>(r) * C);
+        sp.load(p.g, sd + static_cast<int64_t>(r) * C);
+      },
+      [&](P& p, int r) {
+        ct xv[VE], gv[VE];
+        p.x.unpack(xv);
+        p.g.unpack(gv);
 #pragma unroll
-  for (int i = 0; i < VE; ++i) {
-    mu[i] = s[i] = w[i] = b[i] = m1[i] = m2[i] = 0;
-    if (i < count) {
-      const int g = (c0 + i) / cpg;
-      mu[i] = mean[sg + g];
-      s[i] = rstd[sg + g];
-      w[i] = load_param<T>(weight, pl + c0 + i, wide != 0);
-      if (ACT != kGnNone) b[i] = load_param<T>(bias, pl + c0 + i, wide != 0);
-      m1[i] = lds_m1[g];
-      m2[i] = lds_m2[g];
-    }
-  }
-  const int64_t base = ch.first_row * C + c0;
-#pragma unroll 4
-  for (int r = r0; r < ch.rows; r += lanes) {
-    Pack<T, VE> px, pg;
-    px.load(x + base + static_cast<int64_t>(r) * C, count);
-    pg.load(grad_out + base + static_cast<int64_t>(r) * C, count);
-    ct xv[VE], gv[VE];
-    px.unpack(xv);
-    pg.unpack(gv);
-#pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const ct u = (xv[i] - mu[i]) * s[i];
-      const ct dz = ACT == kGnNone ? gv[i] : gv[i] * gn_slope<ACT>(u * w[i] + b[i]);
-      gv[i] = s[i] * (w[i] * dz - m1[i] - u * m2[i]);
-    }
-    pg.pack(gv);
-    pg.store(grad_x + base + static_cast<int64_t>(r) * C, count);
-  }
+        for (int i = 0; i < VE; ++i) {
+          const ct u = (xv[i] - mu[i]) * s[i];
+          ct dz = gv[i];
+          if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[i] + b[i]);
+          gv[i] = s[i] * (w[i] * dz - a1[i] - u * a2[i]);
+        }
+        p.g.pack(gv);
+        sp.store(p.g, dst + static_cast<int64_t>(r) * C);
+      });
 }
 
 }  // namespace msda

@@ -39,6 +39,7 @@ constexpr int64_t kMaxRowBytes = 16384;  // a row of the normalising kernels
 constexpr int64_t kMaxLevels = 16;
 constexpr int64_t kMaxDropElements = int64_t(1) << 35;
 constexpr int64_t kMaxRows = INT32_MAX;
+constexpr int64_t kMaxMaps = int64_t(1) << 21;  // samples x levels x tiles of 32 groups
 
 // ---- argument checks ------------------------------------------------------------------------------
 
@@ -161,6 +162,9 @@ void check_group_norm(const Tensor& x, const Tensor& weight, const Tensor& bias,
   for (int64_t r : rows) positions += r;
   TORCH_CHECK_VALUE(positions == 0 || x.size(0) <= kMaxRows / positions, kGroup,
                     ": at most 2**31 - 1 positions, got ", x.size(0), " x ", positions);
+  TORCH_CHECK_VALUE(x.size(0) <= kMaxMaps / levels / ((groups + 31) / 32), kGroup,
+                    ": at most 2**21 samples x levels (x tiles of 32 groups), got ", x.size(0), " x ",
+                    levels, " with ", groups, " groups");
 }
 
 void check_grad(const char* what, const Tensor& grad, const Tensor& like) {
