@@ -308,6 +308,9 @@ PYRAMIDS = {
     "tall": (1, [(64, 64), (32, 32), (16, 16), (8, 8)], 256, 32),
     "batch": (16, [(4, 4)], 32, 8),
     "narrow": (2, [(40, 50)], 4, 2),
+    # levels that no workgroup holds, next to one row: whole vectors, parts of vectors
+    "long": (2, [(96, 130), (1, 1)], 64, 8),
+    "long_odd": (1, [(96, 130), (2, 1)], 22, 2),
 }
 
 

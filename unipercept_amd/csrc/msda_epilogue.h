@@ -346,8 +346,94 @@ int gn_backward(const GnCall& a, const GnPlan& plan) {
   return run.rc;
 }
 
+// A slab of whole groups for the one-launch kernels, and the threads of its workgroup; false where a
+// level does not fit or the call is too large for slabs of 64 bytes a row (they use half of each
+// cache line).  One launch against three (MI355X, 256 bf16 channels, forward and backward, us):
+// 512 rows 9.9 + 10.3 against 11.2 + 12.6, 64 x 256 rows 10.6 + 16.0 against 13.9 + 17.9; with four
+// vectors a thread it loses (8 x 1024 rows 11.7 + 16.9 against 12.0 + 14.3), so does a slab of 32
+// bytes (17.5 for the latter), and so do 128 x 1024 rows of 512 channels (118 + 184 against 74 + 130).
+constexpr int64_t kGnSmallBytes = 16 << 20;
+inline bool gn_small_plan(const GnPlan& plan, int N, int C, int G, size_t esize, GnSlab* sl,
+                          int* threads) {
+  const int VE = 16 / static_cast<int>(esize), cpg = C / G, S = plan.sums.row_start[plan.sums.levels];
+  if (static_cast<int64_t>(N) * S * C * static_cast<int64_t>(esize) > kGnSmallBytes) return false;
+  int longest = 0;
+  for (int l = 0; l < plan.sums.levels; ++l) {
+    const int rows = plan.sums.row_start[l + 1] - plan.sums.row_start[l];
+    longest = rows > longest ? rows : longest;
+  }
+  int best = 0;
+  for (int k = 1; k <= G && static_cast<int64_t>(k) * cpg <= kGnSlabChannels && best == 0; ++k) {
+    const int vecs = k * cpg / VE;
+    if (G % k == 0 && k * cpg % VE == 0 && (vecs >= 4 || k == G)) best = k;
+  }
+  if (best == 0 || longest > 1024 / (best * cpg / VE) * kGnHold ||
+      static_cast<int64_t>(N) * plan.sums.levels * (G / best) > (1 << 21))
+    return false;
+  *sl = {best, best * cpg, best * cpg / VE, G / best};
+  *threads = 1024;
+  for (int t = 256; t < 1024; t *= 2)
+    if (longest <= t / sl->vecs * kGnHold) {
+      *threads = t;
+      break;
+    }
+  return true;
+}
+
+template <typename T, int ACT>
+int gn_small_forward(const GnCall& a, const GnPlan& plan, const GnSlab& sl, int threads) {
+  Launches run;
+  const size_t lds = (static_cast<size_t>(threads / sl.vecs) * (sl.channels + 1) + 2 * sl.groups) * 4;
+  run((gn_small_kernel<T, ACT>), dim3(a.N * plan.sums.levels * sl.slabs), dim3(threads), lds, a.stream,
+      static_cast<const T*>(a.x), a.weight, a.bias, static_cast<T*>(a.out), static_cast<float*>(a.mean),
+      static_cast<float*>(a.rstd), plan.sums, sl, a.C, a.G, plan.param_levels, static_cast<float>(a.eps),
+      a.wide ? 1 : 0);
+  return run.rc;
+}
+
+template <typename T, int ACT>
+int gn_small_backward(const GnCall& a, const GnPlan& plan, const GnSlab& sl, int threads) {
+  Launches run;
+  const bool params = a.grad_weight != nullptr;
+  const bool direct = a.N == 1 && plan.param_levels == plan.sums.levels;
+  float* partial = params && !direct ? static_cast<float*>(a.workspace) : nullptr;
+  const size_t lds = (static_cast<size_t>(threads / sl.vecs) * (sl.channels + 1) + 2 * sl.channels +
+                      2 * sl.groups) * 4;
+  run((gn_small_bwd_kernel<T, ACT>), dim3(a.N * plan.sums.levels * sl.slabs), dim3(threads), lds, a.stream,
+      static_cast<const T*>(a.grad_out), static_cast<const T*>(a.x), a.weight, a.bias,
+      static_cast<const float*>(a.mean), static_cast<const float*>(a.rstd), static_cast<T*>(a.grad_x),
+      partial, a.grad_weight, a.grad_bias, plan.sums, sl, a.C, a.G, plan.param_levels, a.wide ? 1 : 0);
+  if (partial != nullptr) {
+    // partial rows lie sample by sample, level by level
+    ColumnRuns runs{};
+    runs.outer = a.N;
+    runs.pitch = plan.sums.levels;
+    if (plan.param_levels == 1) {
+      runs.end[0] = plan.sums.levels;
+    } else {
+      for (int l = 0; l < plan.sums.levels; ++l) {
+        runs.begin[l] = l;
+        runs.end[l] = l + 1;
+      }
+    }
+    run((gn_bwd_join_kernel<T>), dim3((a.C + 15) / 16 * 2 * plan.param_levels), dim3(1024), 0, a.stream,
+        static_cast<const float*>(nullptr), static_cast<const float*>(partial),
+        static_cast<float*>(nullptr), static_cast<float*>(nullptr), a.grad_weight, a.grad_bias, plan.sums,
+        runs, 0, a.C, a.G, a.wide ? 1 : 0);
+  }
+  return run.rc;
+}
+
 template <typename T, int ACT>
 int gn_act_run(const GnCall& a, const GnPlan& plan, bool backward) {
+  // (fp64 is for checking gradients: it takes the general kernels)
+  if constexpr (sizeof(T) <= 4) {
+    GnSlab sl;
+    int threads;
+    if (gn_small_plan(plan, a.N, a.C, a.G, sizeof(T), &sl, &threads))
+      return backward ? gn_small_backward<T, ACT>(a, plan, sl, threads)
+                      : gn_small_forward<T, ACT>(a, plan, sl, threads);
+  }
   switch (row_mode(a.C, 16 / static_cast<int>(sizeof(T)))) {
     case kRowEven:
       return backward ? gn_backward<T, ACT, kRowEven>(a, plan) : gn_forward<T, ACT, kRowEven>(a, plan);

@@ -75,34 +75,7 @@ __device__ __forceinline__ void gn_rows(int r0, int rows, int lanes, Load load, 
   }
 }
 
-// (count, mean, M2) of a union of two sets (T. F. Chan, G. H. Golub, R. J. LeVeque 1979)
-template <typename CT>
-struct Moments {
-  CT n, mean, m2;
-  __device__ __forceinline__ void add(CT on, CT omean, CT om2) {
-    const CT total = n + on;
-    if (total > CT(0)) {
-      const CT d = omean - mean, f = on / total;
-      mean += d * f;
-      m2 += om2 + (d * n) * (d * f);  // (an empty side adds 0 whatever d is)
-      n = total;
-    }
-  }
-};
-
-// over the `width` lanes of a team (a power of two up to the wave)
-template <typename CT>
-__device__ __forceinline__ void team_moments(Moments<CT>& m, int width) {
-  for (int off = 1; off < width; off <<= 1) {
-    const CT on = __shfl_xor(m.n, off, 64), omean = __shfl_xor(m.mean, off, 64),
-             om2 = __shfl_xor(m.m2, off, 64);
-    // both lanes of a pair join in the same order, so that all lanes hold the same bits
-    const bool low = (threadIdx.x & off) == 0;
-    Moments<CT> a{low ? m.n : on, low ? m.mean : omean, low ? m.m2 : om2};
-    a.add(low ? on : m.n, low ? omean : m.mean, low ? om2 : m.m2);
-    m = a;
-  }
-}
+// sums of two values over the `width` lanes of a team (a power of two up to the wave)
 template <typename CT>
 __device__ __forceinline__ void team_add2(CT& a, CT& b, int width) {
   for (int off = 1; off < width; off <<= 1) {
@@ -138,11 +111,31 @@ __device__ __forceinline__ void gn_spread(const CT* __restrict__ src, const Span
 __device__ __forceinline__ float gn_sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + __expf(-z)); }
 __device__ __forceinline__ double gn_sigmoid(double z) { return 1.0 / (1.0 + exp(-z)); }
 
+// Normal distribution function Phi(z) and, with it, exp(-z^2 / 2).  In fp32 by formula 7.1.26 of
+// M. Abramowitz and I. A. Stegun, Handbook of Mathematical Functions (erf to 1.5e-7, about two
+// roundings of 1 + erf), which shares its exponential with the density.
+__device__ __forceinline__ float gn_phi(float z, float& e) {
+  const float a = fabsf(z) * 0.70710678118654752440f;
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * a);
+  e = __expf(-a * a);
+  const float poly =
+      t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  const float upper = 0.5f * poly * e;  // 1 - Phi(|z|)
+  return z < 0.f ? upper : 1.f - upper;
+}
+__device__ __forceinline__ double gn_phi(double z, double& e) {
+  e = exp(z * z * -0.5);
+  return 0.5 * erfc(z * -0.70710678118654752440);
+}
+
 template <int ACT, typename CT>
 __device__ __forceinline__ CT gn_act(CT z) {
   if constexpr (ACT == kGnRelu) return z <= CT(0) ? CT(0) : z;  // NaN stays
   if constexpr (ACT == kGnSilu) return z * gn_sigmoid(z);
-  if constexpr (ACT == kGnGelu) return CT(0.5) * z * (CT(1) + erf(z * CT(0.70710678118654752440)));
+  if constexpr (ACT == kGnGelu) {
+    CT e;
+    return z * gn_phi(z, e);
+  }
   return z;
 }
 
@@ -154,8 +147,9 @@ __device__ __forceinline__ CT gn_slope(CT z) {
     return s * (CT(1) + z * (CT(1) - s));
   }
   if constexpr (ACT == kGnGelu) {
-    const CT below = CT(0.5) * (CT(1) + erf(z * CT(0.70710678118654752440)));
-    return below + z * exp(z * z * CT(-0.5)) * CT(0.39894228040143267794);
+    CT e;
+    const CT phi = gn_phi(z, e);
+    return phi + z * e * CT(0.39894228040143267794);
   }
   return CT(1);
 }
@@ -182,26 +176,24 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(
   const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
   for (int k = threadIdx.x - r0 * vecs; k < vecs && r0 < lanes; k += kGnThreads) {
     const auto sp = Span<VE, MODE>::at(k, C);
+    // about the first row; a step has kGnRowsAhead rows in flight, the first row among them
     ct pivot[VE], s[VE], q[VE];
 #pragma unroll
     for (int i = 0; i < VE; ++i) pivot[i] = s[i] = q[i] = 0;
-    if (r0 < ch.rows) {
-      P p;
-      sp.load(p, src + static_cast<int64_t>(r0) * C);
-      p.unpack(pivot);
-    }
+    bool first = true;
     gn_rows<P>(
-        r0 + lanes, ch.rows, lanes,
-        [&](P& p, int r) { sp.load(p, src + static_cast<int64_t>(r) * C); },
+        r0, ch.rows, lanes, [&](P& p, int r) { sp.load(p, src + static_cast<int64_t>(r) * C); },
         [&](P& p, int) {
           ct v[VE];
           p.unpack(v);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
+            if (first) pivot[i] = v[i];
             const ct d = v[i] - pivot[i];
             s[i] += d;
             q[i] += d * d;
           }
+          first = false;
         });
     const int n = gn_lane_rows(ch.rows, r0, lanes);
     const ct inv = n > 0 ? ct(1) / static_cast<ct>(n) : ct(0);
@@ -214,19 +206,40 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(
       }
   }
   __syncthreads();
+  // groups: the mean of the parts' means, then M2 about it (sum of the parts' M2 and of
+  // n_r (mean_r - mean)^2), all about one part's mean so that a common offset costs nothing
   const int cpg = C / G, width = gn_team_width(kGnThreads, G), teams = kGnThreads / width;
-  const int j = threadIdx.x & (width - 1);
+  const int j = threadIdx.x & (width - 1), parts = min(lanes, ch.rows) * cpg;
+  const ct share = ct(1) / (static_cast<ct>(ch.rows) * static_cast<ct>(cpg));
+  const int full = ch.rows / lanes, rest = ch.rows - full * lanes;  // rows of lane r: full, or one more
+  const int step_r = width / cpg, step_c = width - step_r * cpg, r_at = j / cpg, c_at = j - r_at * cpg;
   for (int g = threadIdx.x / width; g < G; g += teams) {
-    Moments<ct> m{0, 0, 0};
-    for (int e = j; e < lanes * cpg; e += width) {
-      const int r = e / cpg, at = r * C + g * cpg + (e - r * cpg);
-      m.add(static_cast<ct>(gn_lane_rows(ch.rows, r, lanes)), lds_mean[at], lds_m2[at]);
-    }
-    team_moments(m, width);
+    const ct pivot = lds_mean[g * cpg];
+    // visits part e = j, j + width, ... as (row lane, channel), without a division each
+    auto visit = [&](auto f) {
+      int r = r_at, c = c_at;
+      for (int e = j; e < parts; e += width) {
+        f(r * C + g * cpg + c, static_cast<ct>(full + (r < rest ? 1 : 0)));
+        r += step_r;
+        c += step_c;
+        if (c >= cpg) {
+          c -= cpg;
+          ++r;
+        }
+      }
+    };
+    ct mu = 0, m2 = 0;
+    visit([&](int at, ct n) { mu += n * share * (lds_mean[at] - pivot); });
+    for (int off = 1; off < width; off <<= 1) mu += __shfl_xor(mu, off, 64);
+    visit([&](int at, ct n) {
+      const ct d = lds_mean[at] - pivot - mu;
+      m2 += lds_m2[at] + n * d * d;
+    });
+    for (int off = 1; off < width; off <<= 1) m2 += __shfl_xor(m2, off, 64);
     if (j == 0) {
       ct* dst = partial + (static_cast<int64_t>(blockIdx.x) * G + g) * 2;
-      dst[0] = m.mean;
-      dst[1] = m.m2;
+      dst[0] = pivot + mu;
+      dst[1] = m2;
     }
   }
 }
@@ -501,6 +514,261 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(
         p.g.pack(gv);
         sp.store(p.g, dst + static_cast<int64_t>(r) * C);
       });
+}
+
+// ---- small levels: one launch --------------------------------------------------------------------
+// Where every level of the call fits the registers of a workgroup per slab of whole groups, the
+// workgroup reads its slab once, forms the sums and writes: one launch instead of three and one
+// reading instead of two.  A thread holds up to kGnHold vectors of each tensor; statistics are taken
+// in two passes over them (mean, then squares about it).
+// Slabs are whole vectors wide.  blockDim.x is chosen by the host (up to 1024).
+constexpr int kGnHold = 2;
+constexpr int kGnSlabChannels = 256;  // widest slab: no more channels than threads
+
+struct GnSlab {
+  int groups, channels, vecs;  // of a slab
+  int slabs;                   // of a row
+};
+
+struct GnSmall {
+  int n, level, slab, rows, lanes, r0, count;
+  int64_t base;  // of the thread's first vector
+};
+
+__device__ __forceinline__ GnSmall gn_small(const GnCut& cut, const GnSlab& sl, int C, int VE) {
+  GnSmall s;
+  const int cell = blockIdx.x / sl.slabs;
+  s.slab = blockIdx.x - cell * sl.slabs;
+  s.n = cell / cut.levels;
+  s.level = cell - s.n * cut.levels;
+  s.rows = cut.row_start[s.level + 1] - cut.row_start[s.level];
+  s.lanes = blockDim.x / sl.vecs;
+  s.r0 = threadIdx.x / sl.vecs;
+  s.count = s.r0 < s.lanes ? gn_lane_rows(s.rows, s.r0, s.lanes) : 0;
+  const int64_t row = static_cast<int64_t>(s.n) * cut.row_start[cut.levels] + cut.row_start[s.level] + s.r0;
+  s.base = row * C + s.slab * sl.channels + (threadIdx.x - s.r0 * sl.vecs) * VE;
+  return s;
+}
+
+// Sum over rows of what every thread holds per channel of the slab, in two steps: the threads' VE
+// values to LDS (`lanes` rows of channels + 1: the odd pitch keeps columns off one bank), then
+// blockDim / channels threads a column.  Leaves gn_small_parts() rows of sums at the start of `lds`,
+// which the caller adds up after the last barrier.
+__device__ __forceinline__ int gn_small_parts(const GnSmall& s, const GnSlab& sl) {
+  return min(static_cast<int>(blockDim.x) / sl.channels, min(s.lanes, s.rows));
+}
+template <int VE>
+__device__ __forceinline__ void gn_small_columns(const float (&v)[VE], const GnSmall& s, const GnSlab& sl,
+                                                 float* lds) {
+  const int pitch = sl.channels + 1, c0 = (threadIdx.x - s.r0 * sl.vecs) * VE;
+  if (s.r0 < s.lanes) {
+#pragma unroll
+    for (int i = 0; i < VE; ++i) lds[s.r0 * pitch + c0 + i] = v[i];
+  }
+  __syncthreads();
+  const int parts = gn_small_parts(s, sl), part = threadIdx.x / sl.channels;
+  const int c = threadIdx.x - part * sl.channels, used = min(s.lanes, s.rows);
+  float sum = 0;
+  if (part < parts)
+    for (int r = part; r < used; r += parts) sum += lds[r * pitch + c];
+  __syncthreads();
+  if (part < parts) lds[part * pitch + c] = sum;
+  __syncthreads();
+}
+
+// per group; `totals` (groups of the slab) receives the sums
+template <int VE>
+__device__ __forceinline__ void gn_small_sum(const float (&v)[VE], const GnSmall& s, const GnSlab& sl, int cpg,
+                                             float* lds, float* totals) {
+  gn_small_columns<VE>(v, s, sl, lds);
+  const int pitch = sl.channels + 1, parts = gn_small_parts(s, sl);
+  const int width = gn_team_width(blockDim.x, sl.groups), teams = blockDim.x / width;
+  const int j = threadIdx.x & (width - 1);
+  for (int g = threadIdx.x / width; g < sl.groups; g += teams) {
+    float sum = 0;
+    for (int q = j; q < parts; q += width)
+      for (int c = 0; c < cpg; ++c) sum += lds[q * pitch + g * cpg + c];
+    for (int off = 1; off < width; off <<= 1) sum += __shfl_xor(sum, off, 64);
+    if (j == 0) totals[g] = sum;
+  }
+  __syncthreads();
+}
+
+// mean and rstd (N, levels, G) may be NULL.  Dynamic LDS: lanes * (channels + 1) + 2 * groups values.
+template <typename T, int ACT>
+__global__ __launch_bounds__(1024) void gn_small_kernel(
+    const T* __restrict__ x, const void* __restrict__ weight, const void* __restrict__ bias,
+    T* __restrict__ out, float* __restrict__ mean, float* __restrict__ rstd, GnCut cut, GnSlab sl, int C,
+    int G, int param_levels, float eps, int wide) {
+  constexpr int VE = 16 / sizeof(T);
+  extern __shared__ __align__(16) char gn_lds[];
+  float* lds = reinterpret_cast<float*>(gn_lds);
+  const GnSmall s = gn_small(cut, sl, C, VE);
+  const int cpg = C / G;
+  float* totals = lds + s.lanes * (sl.channels + 1);
+  const int64_t step = static_cast<int64_t>(s.lanes) * C;
+  Pack<T, VE> p[kGnHold];
+#pragma unroll
+  for (int i = 0; i < kGnHold; ++i)
+    if (i < s.count) p[i].template load<false>(x + s.base + i * step);
+  float sum[VE], mu[VE], a[VE], b[VE];
+#pragma unroll
+  for (int e = 0; e < VE; ++e) sum[e] = 0;
+#pragma unroll
+  for (int i = 0; i < kGnHold; ++i)
+    if (i < s.count) {
+      float v[VE];
+      p[i].unpack(v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[e] += v[e];
+    }
+  gn_small_sum<VE>(sum, s, sl, cpg, lds, totals);
+  const float inv = 1.f / (static_cast<float>(s.rows) * static_cast<float>(cpg));
+  const Span<VE, kRowEven> sp = {static_cast<int>((threadIdx.x - s.r0 * sl.vecs) * VE), 0, VE};
+  gn_spread(totals, sp, cpg, mu);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) {
+    mu[e] *= inv;
+    sum[e] = 0;
+  }
+#pragma unroll
+  for (int i = 0; i < kGnHold; ++i)
+    if (i < s.count) {
+      float v[VE];
+      p[i].unpack(v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) sum[e] += (v[e] - mu[e]) * (v[e] - mu[e]);
+    }
+  float* squares = totals + sl.groups;
+  gn_small_sum<VE>(sum, s, sl, cpg, lds, squares);
+  const int64_t cell = (static_cast<int64_t>(s.n) * cut.levels + s.level) * G + s.slab * sl.groups;
+  if (mean != nullptr)
+    for (int g = threadIdx.x; g < sl.groups; g += blockDim.x) {
+      mean[cell + g] = totals[g] * inv;
+      rstd[cell + g] = 1.f / sqrtf(squares[g] * inv + eps);
+    }
+  gn_spread(squares, sp, cpg, a);
+  const int64_t pc = (param_levels > 1 ? static_cast<int64_t>(s.level) * C : 0) + s.slab * sl.channels;
+  float w[VE];
+  load_params<T>(weight, pc, sp, wide != 0, w);
+  load_params<T>(bias, pc, sp, wide != 0, b);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) a[e] = w[e] / sqrtf(a[e] * inv + eps);
+#pragma unroll
+  for (int i = 0; i < kGnHold; ++i)
+    if (i < s.count) {
+      float v[VE];
+      p[i].unpack(v);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) v[e] = gn_act<ACT>((v[e] - mu[e]) * a[e] + b[e]);
+      p[i].pack(v);
+      p[i].template store<false>(out + s.base + i * step);
+    }
+}
+
+// partial (one row of 2 C sums per (sample, level): dz * u, then dz) or, with `direct`, the gradients
+// themselves (one sample, parameters per level); grad_weight NULL: neither.  grad_x may be NULL.
+template <typename T, int ACT>
+__global__ __launch_bounds__(1024) void gn_small_bwd_kernel(
+    const T* __restrict__ grad_out, const T* __restrict__ x, const void* __restrict__ weight,
+    const void* __restrict__ bias, const float* __restrict__ mean, const float* __restrict__ rstd,
+    T* __restrict__ grad_x, float* __restrict__ partial, void* __restrict__ grad_weight,
+    void* __restrict__ grad_bias, GnCut cut, GnSlab sl, int C, int G, int param_levels, int wide) {
+  constexpr int VE = 16 / sizeof(T), HOLD = kGnHold;
+  extern __shared__ __align__(16) char gn_lds[];
+  float* lds = reinterpret_cast<float*>(gn_lds);
+  const GnSmall s = gn_small(cut, sl, C, VE);
+  const int cpg = C / G, pitch = sl.channels + 1;
+  float* columns = lds + s.lanes * pitch;  // dw, db of the slab's channels
+  float* totals = columns + 2 * sl.channels;
+  const int64_t step = static_cast<int64_t>(s.lanes) * C;
+  Pack<T, VE> px[HOLD], pg[HOLD];
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (i < s.count) {
+      px[i].template load<false>(x + s.base + i * step);
+      pg[i].template load<false>(grad_out + s.base + i * step);
+    }
+  const int c0 = (threadIdx.x - s.r0 * sl.vecs) * VE;
+  const Span<VE, kRowEven> sp = {c0, 0, VE};
+  const int64_t cell = (static_cast<int64_t>(s.n) * cut.levels + s.level) * G + s.slab * sl.groups;
+  const int64_t pc = (param_levels > 1 ? static_cast<int64_t>(s.level) * C : 0) + s.slab * sl.channels;
+  float mu[VE], r[VE], w[VE], b[VE], sums[2][VE];
+  gn_spread(mean + cell, sp, cpg, mu);
+  gn_spread(rstd + cell, sp, cpg, r);
+  load_params<T>(weight, pc, sp, wide != 0, w);
+  load_params<T>(bias, pc, sp, wide != 0, b);
+#pragma unroll
+  for (int e = 0; e < VE; ++e) sums[0][e] = sums[1][e] = 0;
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (i < s.count) {
+      float xv[VE], gv[VE];
+      px[i].unpack(xv);
+      pg[i].unpack(gv);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float u = (xv[e] - mu[e]) * r[e];
+        float dz = gv[e];
+        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[e] + b[e]);
+        sums[0][e] += dz * u;
+        sums[1][e] += dz;
+      }
+    }
+  const int parts = gn_small_parts(s, sl);
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    gn_small_columns<VE>(sums[k], s, sl, lds);
+    for (int c = threadIdx.x; c < sl.channels; c += blockDim.x) {
+      float sum = 0;
+      for (int q = 0; q < parts; ++q) sum += lds[q * pitch + c];
+      columns[k * sl.channels + c] = sum;
+    }
+    __syncthreads();
+  }
+  const int64_t slot = static_cast<int64_t>(s.n) * cut.levels + s.level;
+  if (grad_weight != nullptr)
+    for (int c = threadIdx.x; c < sl.channels; c += blockDim.x) {
+      if (partial != nullptr) {
+        partial[slot * 2 * C + s.slab * sl.channels + c] = columns[c];
+        partial[(slot * 2 + 1) * C + s.slab * sl.channels + c] = columns[sl.channels + c];
+      } else {
+        store_param<T>(grad_weight, pc + c, columns[c], wide != 0);
+        store_param<T>(grad_bias, pc + c, columns[sl.channels + c], wide != 0);
+      }
+    }
+  if (grad_x == nullptr) return;
+  const float inv = 1.f / (static_cast<float>(s.rows) * static_cast<float>(cpg));
+  for (int g = threadIdx.x; g < sl.groups; g += blockDim.x) {
+    float m1 = 0, m2 = 0;
+    for (int c = g * cpg; c < (g + 1) * cpg; ++c) {
+      const float wc = load_param<T>(weight, pc + c, wide != 0);
+      m1 += columns[sl.channels + c] * wc;
+      m2 += columns[c] * wc;
+    }
+    totals[g] = m1 * inv;
+    totals[sl.groups + g] = m2 * inv;
+  }
+  __syncthreads();
+  float m1[VE], m2[VE];
+  gn_spread(totals, sp, cpg, m1);
+  gn_spread(totals + sl.groups, sp, cpg, m2);
+#pragma unroll
+  for (int i = 0; i < HOLD; ++i)
+    if (i < s.count) {
+      float xv[VE], gv[VE];
+      px[i].unpack(xv);
+      pg[i].unpack(gv);
+#pragma unroll
+      for (int e = 0; e < VE; ++e) {
+        const float u = (xv[e] - mu[e]) * r[e];
+        float dz = gv[e];
+        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[e] + b[e]);
+        gv[e] = r[e] * (w[e] * dz - m1[e] - u * m2[e]);
+      }
+      pg[i].pack(gv);
+      pg[i].template store<false>(grad_x + s.base + i * step);
+    }
 }
 
 }  // namespace msda
