@@ -629,6 +629,133 @@ def test_group_norm_beyond_32_bit_offsets():
     assert ((z[-3:].float().cpu() - want).abs() <= 2.0**-8 * want.abs() + 1e-4).all()
 
 
+def test_gradients_beyond_32_bit_offsets():
+    """The last rows of gradients of more than 2^31 elements have the bits of the rows alone."""
+    c, rows = 4096, (1 << 19) + 64
+    g = torch.Generator(device="cuda").manual_seed(1)
+    tail = 64  # (a multiple of every team's step: the last rows fall into workgroups of their own)
+    x = torch.empty(rows, c, dtype=BF16, device="cuda").normal_(generator=g)
+    dy = torch.empty(rows, c, dtype=BF16, device="cuda").normal_(generator=g)
+    w = torch.ones(c, device="cuda")
+    op = torch.ops.unipercept
+    _, mean, rstd = op.dropout_add_norm_fwd(x, x, w, w, None, 0.0, 0, 1e-5, True)
+    gx, gr, gw, gb = op.dropout_add_norm_bwd(dy, x, x, w, mean, rstd, rng(), 0.5, 1, True, True, True)
+    one = op.dropout_add_norm_bwd(
+        dy[-tail:], x[-tail:], x[-tail:], w, mean[-tail:], rstd[-tail:], None, 0.0, 0, True, True, True)
+    keep = torch.from_numpy(ref.keep((rows - tail) * c, tail * c, 0.5, *STATE, 1)).view(tail, c).cuda()
+    assert torch.equal(gx[-tail:] != 0, keep & (gr[-tail:] != 0)) and torch.isfinite(gw).all()
+    del gx, gr
+    _, gr, _, _ = op.dropout_add_norm_bwd(dy, x, x, w, mean, rstd, None, 0.0, 0, False, True, False)
+    assert torch.equal(gr[-tail:], one[1])
+    want = dy.float().sum(0)
+    assert (gb - want).norm() <= 1e-4 * want.norm()
+    del gr, gb
+    y = op.counter_dropout_fwd(x, rng(), 0.5, 2, "relu")
+    gx = op.counter_dropout_bwd(dy, y, None, 0.5, 2, "relu")
+    assert torch.equal(gx[-tail:], torch.where(y[-tail:] > 0, dy[-tail:] * 2, torch.zeros_like(dy[-tail:])))
+    del y, gx
+    # group norm: the last sample of several against the sample alone
+    n = 4
+    x, dy = x[: rows // n * n].view(n, rows // n, c), dy[: rows // n * n].view(n, rows // n, c)
+    _, mean, rstd = op.level_group_norm_fwd(x, w, w, 32, [], 1e-5, "silu", True)
+    gx, gw, gb = op.level_group_norm_bwd(dy, x, w, w, mean, rstd, 32, [], "silu", True, True)
+    last = op.level_group_norm_bwd(dy[-1:], x[-1:], w, w, mean[-1:], rstd[-1:], 32, [], "silu", True, True)
+    # (chunks differ with the batch: fp32 sums in another order, one step of bf16)
+    assert ((gx[-1:].float() - last[0].float()).abs() <= 2.0**-7 * last[0].float().abs() + 1e-6).all()
+
+
+@pytest.mark.parametrize("dtype,c,groups", [(BF16, 8192, 1), (F16, 8191, 1), (F32, 4096, 1), (F32, 4095, 3), (F64, 2047, 1),
+                                            (BF16, 8192, 8192), (F32, 4096, 32)])
+def test_group_norm_widest_rows(dtype, c, groups):
+    PYRAMIDS["_widest"] = (2, [(3, 3), (1, 2)], c, groups)
+    try:
+        run_group("_widest", dtype, F64 if dtype == F64 else F32, "silu")
+    finally:
+        del PYRAMIDS["_widest"]
+
+
+def test_group_norm_many_samples():
+    """More (sample, level) pairs than rows in each, through the one-launch and the general kernels."""
+    for n, levels, c, groups in ((5000, [(1, 2), (1, 1)], 16, 4), (3000, [(1, 3)], 6, 3), (4000, [(4, 4)], 256, 32)):
+        x = normal((n, sum(h * w for h, w in levels), c), F32, n)
+        w, b = normal((len(levels), c), F32, 2), normal((len(levels), c), F32, 3)
+        rows = [h * v for h, v in levels]
+        want, _ = ref.group_norm(x, w, b, groups, rows, 1e-5, "none")
+        got = level_group_norm(x.cuda(), w.cuda(), b.cuda(), groups, levels).cpu().double()
+        # groups of a few elements: a step of fp32 in x - mean against spreads down to 1e-3
+        assert ((got - want).abs() <= 2.0**-24 * 1e4 * (1 + want.abs())).all()
+
+
+def test_no_memory_is_kept_between_steps():
+    calls, _ = _calls()
+    for call in calls.values():
+        call()
+    torch.cuda.synchronize()
+    before = torch.cuda.memory_allocated()
+    for _ in range(5):
+        for call in calls.values():
+            call()
+    torch.cuda.synchronize()
+    assert torch.cuda.memory_allocated() == before
+
+
+def test_inference_mode_and_detached_results():
+    x, w, b = normal((2, 20, 64), F32, 1).cuda(), torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    w.requires_grad_(True)
+    want = [counter_dropout(x, 0.3, rng(), 0, "relu"), dropout_add_layer_norm(x, x, w, b, 0.3, rng()),
+            level_group_norm(x, w, b, 8)]
+    assert [t.requires_grad for t in want] == [False, True, True]
+    for mode in (torch.inference_mode, torch.no_grad):
+        with mode():
+            got = [counter_dropout(x, 0.3, rng(), 0, "relu"), dropout_add_layer_norm(x, x, w, b, 0.3, rng()),
+                   level_group_norm(x, w, b, 8)]
+        assert all(torch.equal(a, c) for a, c in zip(got, want)) and not any(t.requires_grad for t in got)
+
+
+def test_function_transforms_are_right_or_refused():
+    """torch.func.grad either gives the gradient or raises: never a silent zero."""
+    x = normal((4, 64), F32, 1).cuda()
+    w, b = torch.ones(64, device="cuda"), torch.zeros(64, device="cuda")
+    state = rng()
+    for f in (lambda t: counter_dropout(t, 0.3, state, 0), lambda t: dropout_add_layer_norm(t, t, w, b),
+              lambda t: level_group_norm(t[:, None], w, b, 8)):
+        leaf = x.clone().requires_grad_(True)
+        (want,) = torch.autograd.grad(f(leaf).square().sum(), leaf)
+        try:
+            got = torch.func.grad(lambda t: f(t).square().sum())(x)
+        except RuntimeError:
+            continue
+        assert torch.equal(got, want)
+
+
+def test_two_threads_at_once():
+    """Calls of two host threads on streams of their own."""
+    import threading
+
+    calls, _ = _calls()
+    want = {name: call() for name, call in calls.items()}
+    torch.cuda.synchronize()
+    results, errors = [], []
+
+    def work():
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(10):
+                    results.append({name: call() for name, call in calls.items()})
+            stream.synchronize()
+        except BaseException as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    [t.start() for t in threads]
+    [t.join() for t in threads]
+    assert not errors and len(results) == 20
+    for got in results:
+        for name in want:
+            assert all(torch.equal(a, c) for a, c in zip(want[name], got[name])), name
+
+
 # ---- the path they were made for ---------------------------------------------------------------------
 
 
