@@ -304,8 +304,9 @@ def test_abi_add_norm_errors():
         assert call(dx=1, dr=1, dp=1, c=2049) == -2  # 16 KiB of the residual's type
     assert fwd(eps=-1.0) == -2 and fwd(eps=float("nan")) == -2
     assert bwd(ws=None) == -5 and bwd(ws=FAKE + 4) == -5 and bwd(nbytes=need(4, 8, 0, 0) - 1) == -5
-    # two sums per column and workgroup; 512 threads take 64 rows of 256 fp32 columns
-    assert need(4, 8, 0, 0) == 2 * 8 * 4 and need(10**6, 256, 2, 0) == 15625 * 2 * 256 * 4
+    # two sums per column and workgroup (512 threads take 32 rows of 256 fp32 columns), and 16 rows
+    # of them for the second step where there are many workgroups
+    assert need(4, 8, 0, 0) == 2 * 8 * 4 and need(10**6, 256, 2, 0) == (31250 + 16) * 2 * 256 * 4
     assert need(4, 8, 1, 1) == 2 * 8 * 8 and need(0, 8, 0, 0) == 0 and need(4, 8, 0, 2) == 0
 
 

@@ -890,6 +890,8 @@ def test_compiled_graphs_hold_the_operators():
         return [out.detach(), *torch.autograd.grad(out.square().sum(), (xs, w, b))]
 
     want = grads(net)
-    got = grads(torch.compile(net, backend="aot_eager", fullgraph=True))
-    for a, c in zip(got, want):
-        assert torch.equal(a, c)
+    for dynamic in (False, True):
+        torch._dynamo.reset()
+        got = grads(torch.compile(net, backend="aot_eager", fullgraph=True, dynamic=dynamic))
+        for a, c in zip(got, want):
+            assert torch.equal(a, c)

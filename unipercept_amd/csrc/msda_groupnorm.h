@@ -358,15 +358,19 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(
   const int r0 = vecs < kGnThreads ? threadIdx.x / vecs : 0;
   for (int k = threadIdx.x - r0 * vecs; k < vecs && r0 < lanes; k += kGnThreads) {
     const auto sp = Span<VE, MODE>::at(k, C);
-    ct mu[VE], s[VE], w[VE], b[VE], dw[VE], db[VE];
+    // d = x - mu, z = d * (s w) + b; s * sum dz d is the sum of dz u
+    ct mu[VE], s[VE], a[VE] = {}, b[VE] = {}, dw[VE], db[VE];
     gn_spread(mean + sg, sp, cpg, mu);
     gn_spread(rstd + sg, sp, cpg, s);
     if constexpr (ACT != kGnNone) {
-      load_params<T>(weight, pl, sp, wide != 0, w);
+      load_params<T>(weight, pl, sp, wide != 0, a);
       load_params<T>(bias, pl, sp, wide != 0, b);
     }
 #pragma unroll
-    for (int i = 0; i < VE; ++i) dw[i] = db[i] = 0;
+    for (int i = 0; i < VE; ++i) {
+      a[i] *= s[i];
+      dw[i] = db[i] = 0;
+    }
     gn_rows<P>(
         r0, ch.rows, lanes,
         [&](P& p, int r) {
@@ -379,17 +383,17 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(
           p.g.unpack(gv);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            const ct u = (xv[i] - mu[i]) * s[i];
+            const ct d = xv[i] - mu[i];
             ct dz = gv[i];
-            if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[i] + b[i]);
-            dw[i] += dz * u;
+            if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(d * a[i] + b[i]);
+            dw[i] += dz * d;
             db[i] += dz;
           }
         });
 #pragma unroll
     for (int i = 0; i < VE; ++i)
       if (sp.owns(i)) {
-        lds_dw[r0 * C + sp.c + i] = dw[i];
+        lds_dw[r0 * C + sp.c + i] = dw[i] * s[i];
         lds_db[r0 * C + sp.c + i] = db[i];
       }
   }

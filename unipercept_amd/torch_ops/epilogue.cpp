@@ -52,6 +52,21 @@ int dtype_code(at::ScalarType t) {
     default: return -1;
   }
 }
+// Sizes as plain numbers.  Under a trace with symbolic shapes the numbers of this call are taken and
+// guarded: a call of other sizes is traced again.
+at::DimVector dims(const Tensor& t) {
+  if (!t.unsafeGetTensorImpl()->has_symbolic_sizes_strides()) return at::DimVector(t.sizes());
+  at::DimVector out;
+  for (const c10::SymInt& s : t.sym_sizes()) out.push_back(s.guard_int(__FILE__, __LINE__));
+  return out;
+}
+int64_t count(const at::DimVector& d) {
+  int64_t n = 1;
+  for (int64_t v : d) n *= v;
+  return n;
+}
+IntArrayRef shown(const at::DimVector& d) { return IntArrayRef(d.data(), d.size()); }
+
 bool half_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
 at::ScalarType compute_type(at::ScalarType t) { return t == at::kDouble ? at::kDouble : at::kFloat; }
 
@@ -75,12 +90,14 @@ void check_rng(const char* what, double p, int64_t site, const Tensor& state, co
   TORCH_CHECK_VALUE(site >= 0 && site <= INT32_MAX, what, ": site must lie in [0, 2**31), got ", site);
   if (p == 0.0) return;
   TORCH_CHECK_VALUE(state.defined(), what, ": p > 0 needs rng_state (see new_rng_state)");
-  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && state.dim() == 1 && state.size(0) == 2, what,
-                    ": rng_state must be an int64 tensor (seed, offset), got ", state.sizes(), " ",
+  const at::DimVector sd = dims(state);
+  TORCH_CHECK_VALUE(state.scalar_type() == at::kLong && sd.size() == 1 && sd[0] == 2, what,
+                    ": rng_state must be an int64 tensor (seed, offset), got ", shown(sd), " ",
                     state.scalar_type());
   TORCH_CHECK(state.device() == x.device(), what, ": rng_state lives on ", state.device(),
               ", the input on ", x.device());
-  TORCH_CHECK_VALUE(x.numel() <= kMaxDropElements, what, ": at most 2**35 elements, got ", x.numel());
+  const int64_t n = count(dims(x));
+  TORCH_CHECK_VALUE(n <= kMaxDropElements, what, ": at most 2**35 elements, got ", n);
 }
 
 void check_row(const char* what, int64_t columns, const Tensor& t) {
@@ -91,7 +108,7 @@ void check_row(const char* what, int64_t columns, const Tensor& t) {
 
 void check_params(const char* what, const Tensor& weight, const Tensor& bias, const Tensor& x,
                   at::ScalarType dtype) {
-  TORCH_CHECK_VALUE(weight.sizes() == bias.sizes() && weight.scalar_type() == bias.scalar_type(), what,
+  TORCH_CHECK_VALUE(dims(weight) == dims(bias) && weight.scalar_type() == bias.scalar_type(), what,
                     ": weight and bias must agree in shape and dtype");
   TORCH_CHECK_TYPE(weight.scalar_type() == dtype ||
                        (half_type(x.scalar_type()) && weight.scalar_type() == at::kFloat),
@@ -109,29 +126,32 @@ void check_add_norm(const Tensor& x, const Tensor& residual, const Tensor& weigh
                     const Tensor& state, double p, int64_t site, double eps) {
   check_tensor(kNorm, x);
   check_tensor(kNorm, residual);
-  TORCH_CHECK_VALUE(x.dim() >= 1 && x.sizes() == residual.sizes(), kNorm,
-                    ": x and residual must agree in shape, got ", x.sizes(), " and ", residual.sizes());
+  const at::DimVector xd = dims(x), wd = dims(weight);
+  TORCH_CHECK_VALUE(!xd.empty() && xd == dims(residual), kNorm,
+                    ": x and residual must agree in shape, got ", shown(xd), " and ",
+                    shown(dims(residual)));
   TORCH_CHECK_TYPE(residual.scalar_type() == x.scalar_type() ||
                        (half_type(x.scalar_type()) && residual.scalar_type() == at::kFloat),
                    kNorm, ": residual must have x's dtype (or float32 next to a 16-bit x), got ",
                    residual.scalar_type(), " next to ", x.scalar_type());
   TORCH_CHECK(residual.device() == x.device(), kNorm, ": all tensors must live on the same device");
-  const int64_t columns = x.size(-1);
+  const int64_t columns = xd.back();
   check_row(kNorm, columns, residual);
-  TORCH_CHECK_VALUE(weight.dim() == 1 && weight.size(0) == columns, kNorm, ": weight and bias must be (",
-                    columns, ",), got ", weight.sizes());
+  TORCH_CHECK_VALUE(wd.size() == 1 && wd[0] == columns, kNorm, ": weight and bias must be (", columns,
+                    ",), got ", shown(wd));
   check_params(kNorm, weight, bias, x, residual.scalar_type());
   TORCH_CHECK_VALUE(eps >= 0.0, kNorm, ": eps must not be negative, got ", eps);
-  TORCH_CHECK_VALUE(x.numel() / columns <= kMaxRows, kNorm, ": at most 2**31 - 1 rows, got ",
-                    x.numel() / columns);
+  TORCH_CHECK_VALUE(count(xd) / columns <= kMaxRows, kNorm, ": at most 2**31 - 1 rows, got ",
+                    count(xd) / columns);
   check_rng(kNorm, p, site, state, x);
 }
 
 // rows of the levels; one level of all positions without a list
 std::vector<int64_t> level_rows(const Tensor& x, IntArrayRef rows) {
-  TORCH_CHECK_VALUE(x.dim() >= 2, kGroup, ": expected (N, ..., C), got ", x.sizes());
+  const at::DimVector xd = dims(x);
+  TORCH_CHECK_VALUE(xd.size() >= 2, kGroup, ": expected (N, ..., C), got ", shown(xd));
   int64_t positions = 1;
-  for (int64_t d = 1; d + 1 < x.dim(); ++d) positions *= x.size(d);
+  for (size_t d = 1; d + 1 < xd.size(); ++d) positions *= xd[d];
   if (rows.empty()) return {positions};
   TORCH_CHECK_VALUE(static_cast<int64_t>(rows.size()) <= kMaxLevels, kGroup, ": 1 to ", kMaxLevels,
                     " levels, got ", rows.size());
@@ -148,22 +168,23 @@ std::vector<int64_t> level_rows(const Tensor& x, IntArrayRef rows) {
 void check_group_norm(const Tensor& x, const Tensor& weight, const Tensor& bias, int64_t groups,
                       const std::vector<int64_t>& rows, double eps) {
   check_tensor(kGroup, x);
-  const int64_t columns = x.size(-1), levels = static_cast<int64_t>(rows.size());
+  const at::DimVector xd = dims(x), wd = dims(weight);
+  const int64_t samples = xd[0], columns = xd.back(), levels = static_cast<int64_t>(rows.size());
   check_row(kGroup, columns, x);
   TORCH_CHECK_VALUE(groups >= 1 && columns % groups == 0, kGroup, ": ", columns,
                     " channels do not divide into ", groups, " groups");
-  const bool shared = weight.dim() == 1 && weight.size(0) == columns;
-  const bool each = weight.dim() == 2 && weight.size(0) == levels && weight.size(1) == columns;
+  const bool shared = wd.size() == 1 && wd[0] == columns;
+  const bool each = wd.size() == 2 && wd[0] == levels && wd[1] == columns;
   TORCH_CHECK_VALUE(shared || each, kGroup, ": weight and bias must be (", columns, ",) or (", levels,
-                    ", ", columns, "), got ", weight.sizes());
+                    ", ", columns, "), got ", shown(wd));
   check_params(kGroup, weight, bias, x, x.scalar_type());
   TORCH_CHECK_VALUE(eps >= 0.0, kGroup, ": eps must not be negative, got ", eps);
   int64_t positions = 0;
   for (int64_t r : rows) positions += r;
-  TORCH_CHECK_VALUE(positions == 0 || x.size(0) <= kMaxRows / positions, kGroup,
-                    ": at most 2**31 - 1 positions, got ", x.size(0), " x ", positions);
-  TORCH_CHECK_VALUE(x.size(0) <= kMaxMaps / levels / ((groups + 31) / 32), kGroup,
-                    ": at most 2**21 samples x levels (x tiles of 32 groups), got ", x.size(0), " x ",
+  TORCH_CHECK_VALUE(positions == 0 || samples <= kMaxRows / positions, kGroup,
+                    ": at most 2**31 - 1 positions, got ", samples, " x ", positions);
+  TORCH_CHECK_VALUE(samples <= kMaxMaps / levels / ((groups + 31) / 32), kGroup,
+                    ": at most 2**21 samples x levels (x tiles of 32 groups), got ", samples, " x ",
                     levels, " with ", groups, " groups");
 }
 
