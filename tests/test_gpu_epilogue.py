@@ -163,7 +163,7 @@ KINDS = {
     "f16_in_f32": (F16, F32, F32),
 }
 ROWS = [(1, 1), (1, 16), (2, 64), (3, 7), (5, 63), (300, 256), (17, 257), (1200, 24), (9, 515), (4, 1000),
-        (3, 1024), (2, 2048), (5, 2047), (1, 130), (4, 4)]
+        (3, 1024), (2, 2048), (5, 2047), (1, 130), (4, 4), (70, 160), (33, 297), (40, 640), (21, 1500)]
 WIDE = {"f32": [(3, 4096), (2, 4095)], "bf16": [(3, 8192), (2, 8191), (2, 4104)], "f64": [(2, 2048), (2, 2047)],
         "f16_in_f32": [(3, 4096), (2, 4093)]}
 

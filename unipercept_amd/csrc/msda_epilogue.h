@@ -90,18 +90,41 @@ inline int add_norm_check(int64_t rows, int C, double p, int site, int dtype_x, 
   return MSDA_OK;
 }
 
-// A team of lanes for a row of `vecs` vectors: the narrowest that covers it.  A wave or less per row
-// needs no barrier, so rows of up to four vectors a lane stay in one wave; longer ones take a
-// workgroup of four waves.
-inline int add_norm_team(int vecs) { return vecs <= 16 ? 16 : vecs <= 32 ? 32 : vecs <= 256 ? 64 : 256; }
+// Lanes of a row's team and vectors of a lane, for rows of `vecs` vectors.  Few lanes with several
+// vectors spend less on sums over lanes; rows of more than 256 vectors take four waves.  Measured on
+// MI355X, 344064 rows of 256 columns, dropout 0.1, forward / backward in us:
+//   fp32 (64 vectors)   64 x 1: 172 / 303   32 x 2: 168 / 316   16 x 4: 168 / 328
+//   bf16 with fp32 res. 64 x 1: 149 / 251   32 x 2: 139 / 252   16 x 4: 141 / 264
+//   bf16 (32 vectors)   32 x 1: 106 / 161   16 x 2:  91 / 178
+// (the backward keeps more of a row in registers and gains less from the shorter sums).
+// Rows between two shapes take one that leaves few lanes empty (fp16, forward, 21502 rows of 520
+// columns, 65 vectors: 64 x 2 19.0, 32 x 3 15.9; of 1030, 129 vectors: 64 x 4 48, 64 x 3 34; of 258,
+// 33 vectors: 64 x 1 15.5, 16 x 3 11.0).
+struct AddNormTeam {
+  int TS, NV;
+};
+inline AddNormTeam add_norm_team(int vecs, bool f64, bool backward) {
+  if (f64) return vecs <= 64 ? AddNormTeam{64, 1} : vecs <= 256 ? AddNormTeam{64, 4} : AddNormTeam{256, 4};
+  if (vecs <= 16) return {16, 1};
+  if (vecs <= 32) return backward ? AddNormTeam{32, 1} : AddNormTeam{16, 2};
+  if (vecs <= 48) return {16, 3};
+  if (vecs <= 64) return backward ? AddNormTeam{64, 1} : AddNormTeam{32, 2};
+  if (vecs <= 96) return {32, 3};
+  if (vecs <= 128) return {64, 2};
+  if (vecs <= 192) return {64, 3};
+  if (vecs <= 256) return {64, 4};
+  if (vecs <= 512) return {256, 2};
+  return {256, 4};
+}
 // threads of a workgroup and rows in flight of a team in the backward
 constexpr int add_norm_bwd_threads(int TS) { return TS > 64 ? 256 : 512; }
 constexpr int add_norm_bwd_rows(int NV) { return NV == 1 ? 2 : 1; }
 
 // Steps of a workgroup of the backward (NR rows a team each): up to kBwdTeamRows rows a team where
 // there are many rows, one step where there are few, so that they spread over the chip.  Longer
-// workgroups leave fewer partial rows and run slower (344064 rows of 256 fp32 columns, kernel and
-// column sums: 2 rows a team 320 + 21 us, 4 rows 296 + 15, 8 rows 310 + 14, 16 rows 330 + 9).
+// workgroups leave fewer partial rows and run slower (344064 rows of 256 fp32 columns, 8 teams of 64
+// lanes, kernel and column sums: 2 rows a team 320 + 21 us, 4 rows 296 + 15, 8 rows 310 + 14, 16 rows
+// 330 + 9).
 constexpr int kBwdTeamRows = 4;
 struct AddNormGrid {
   int steps;
@@ -109,8 +132,9 @@ struct AddNormGrid {
 };
 inline AddNormGrid add_norm_bwd_grid(int64_t rows, int C, int dtype_res) {
   const int VE = 16 / static_cast<int>(elem_size(dtype_res)), vecs = (C + VE - 1) / VE;
-  const int TS = add_norm_team(vecs), NR = add_norm_bwd_rows((vecs + TS - 1) / TS);
-  const int64_t per_step = static_cast<int64_t>(add_norm_bwd_threads(TS) / TS) * NR;
+  const AddNormTeam team = add_norm_team(vecs, dtype_res == MSDA_F64, true);
+  const int NR = add_norm_bwd_rows(team.NV);
+  const int64_t per_step = static_cast<int64_t>(add_norm_bwd_threads(team.TS) / team.TS) * NR;
   const int most = kBwdTeamRows / NR;
   int64_t steps = rows / (per_step * 512);
   steps = steps < 1 ? 1 : steps > most ? most : steps;
@@ -136,18 +160,22 @@ struct AddNormCall {
 };
 
 template <typename XT, typename RT, int TS, int NV, int MODE>
-int add_norm_launch(const AddNormCall& a, bool backward) {
+int add_norm_forward(const AddNormCall& a) {
   using ct = typename Elem<RT>::compute_t;
   Launches run;
-  if (!backward) {
-    constexpr int NR = NV == 1 ? 2 : 1;
-    run((add_norm_fwd_kernel<XT, RT, TS, NV, NR, MODE>), dim3(pass_grid(a.rows, 256 / TS * NR)),
-        dim3(256), 0, a.stream, static_cast<const XT*>(a.x), static_cast<const RT*>(a.res), a.weight,
-        a.bias, static_cast<RT*>(a.out), static_cast<ct*>(a.mean), static_cast<ct*>(a.rstd),
-        a.rng_state, a.rows, a.C, a.drop.threshold, static_cast<ct>(a.drop.scale), a.site,
-        static_cast<ct>(a.eps), a.wide ? 1 : 0);
-    return run.rc;
-  }
+  constexpr int NR = NV == 1 ? 2 : 1;
+  run((add_norm_fwd_kernel<XT, RT, TS, NV, NR, MODE>), dim3(pass_grid(a.rows, 256 / TS * NR)),
+      dim3(256), 0, a.stream, static_cast<const XT*>(a.x), static_cast<const RT*>(a.res), a.weight,
+      a.bias, static_cast<RT*>(a.out), static_cast<ct*>(a.mean), static_cast<ct*>(a.rstd),
+      a.rng_state, a.rows, a.C, a.drop.threshold, static_cast<ct>(a.drop.scale), a.site,
+      static_cast<ct>(a.eps), a.wide ? 1 : 0);
+  return run.rc;
+}
+
+template <typename XT, typename RT, int TS, int NV, int MODE>
+int add_norm_backward(const AddNormCall& a) {
+  using ct = typename Elem<RT>::compute_t;
+  Launches run;
   constexpr int THREADS = add_norm_bwd_threads(TS), NR = add_norm_bwd_rows(NV);
   const AddNormGrid grid = add_norm_bwd_grid(a.rows, a.C, a.dtype_res);
   run((add_norm_bwd_kernel<XT, RT, TS, NV, NR, THREADS, MODE>),
@@ -174,17 +202,38 @@ int add_norm_launch(const AddNormCall& a, bool backward) {
   return run.rc;
 }
 
-// (team sizes: add_norm_team)
 template <typename XT, typename RT, int MODE>
 int add_norm_width(const AddNormCall& a, bool backward) {
   const int vecs = (a.C + AddNormTypes<XT, RT>::VE - 1) / AddNormTypes<XT, RT>::VE;
-  if (vecs <= 16) return add_norm_launch<XT, RT, 16, 1, MODE>(a, backward);
-  if (vecs <= 32) return add_norm_launch<XT, RT, 32, 1, MODE>(a, backward);
-  if (vecs <= 64) return add_norm_launch<XT, RT, 64, 1, MODE>(a, backward);
-  if (vecs <= 128) return add_norm_launch<XT, RT, 64, 2, MODE>(a, backward);
-  if (vecs <= 256) return add_norm_launch<XT, RT, 64, 4, MODE>(a, backward);
-  if (vecs <= 512) return add_norm_launch<XT, RT, 256, 2, MODE>(a, backward);
-  return add_norm_launch<XT, RT, 256, 4, MODE>(a, backward);
+  const AddNormTeam team = add_norm_team(vecs, sizeof(RT) == 8, backward);
+#define MSDA_TEAM(TS, NV)                                                  \
+  case TS * 8 + NV:                                                        \
+    return backward ? add_norm_backward<XT, RT, TS, NV, MODE>(a)           \
+                    : add_norm_forward<XT, RT, TS, NV, MODE>(a)
+  if constexpr (sizeof(RT) == 8) {
+    switch (team.TS * 8 + team.NV) {
+      MSDA_TEAM(64, 1);
+      MSDA_TEAM(64, 4);
+      MSDA_TEAM(256, 4);
+    }
+  } else {
+    switch (team.TS * 8 + team.NV) {
+      MSDA_TEAM(16, 1);
+      MSDA_TEAM(16, 3);
+      MSDA_TEAM(32, 3);
+      MSDA_TEAM(64, 2);
+      MSDA_TEAM(64, 3);
+      MSDA_TEAM(64, 4);
+      MSDA_TEAM(256, 2);
+      MSDA_TEAM(256, 4);
+      case 16 * 8 + 2: return add_norm_forward<XT, RT, 16, 2, MODE>(a);
+      case 32 * 8 + 1: return add_norm_backward<XT, RT, 32, 1, MODE>(a);
+      case 32 * 8 + 2: return add_norm_forward<XT, RT, 32, 2, MODE>(a);
+      case 64 * 8 + 1: return add_norm_backward<XT, RT, 64, 1, MODE>(a);
+    }
+  }
+#undef MSDA_TEAM
+  return MSDA_ESHAPE;  // (a team that add_norm_team does not name)
 }
 
 template <typename XT, typename RT>
@@ -192,7 +241,11 @@ int add_norm_run(const AddNormCall& a, bool backward) {
   switch (row_mode(a.C, AddNormTypes<XT, RT>::VE)) {
     case kRowEven: return add_norm_width<XT, RT, kRowEven>(a, backward);
     case kRowOdd: return add_norm_width<XT, RT, kRowOdd>(a, backward);
-    default: return add_norm_launch<XT, RT, 16, 1, kRowShort>(a, backward);
+    default: {
+      constexpr int TS = sizeof(RT) == 8 ? 64 : 16;
+      return backward ? add_norm_backward<XT, RT, TS, 1, kRowShort>(a)
+                      : add_norm_forward<XT, RT, TS, 1, kRowShort>(a);
+    }
   }
 }
 
