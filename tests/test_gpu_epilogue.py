@@ -862,6 +862,31 @@ def test_projection_and_encoder_train_together():
                            enc(src, shapes, lsi, pos=pos, spatial_shapes_list=levels))
 
 
+def test_projection_gradients_match_convolutions():
+    """Many tokens (the projections' weight gradients by slices), channels-last and plain maps:
+    outputs and gradients against 1 x 1 convolutions and torch's group norm in fp64."""
+    torch.manual_seed(6)
+    proj = LevelInputProjection([24, 40], 64, 16, "silu").cuda()
+    maps = [normal((2, 24, 128, 136), F32, 1).cuda().contiguous(memory_format=torch.channels_last),
+            normal((2, 40, 31, 17), F32, 2).cuda()]
+    dy = normal((2, 128 * 136 + 31 * 17, 64), F32, 3).cuda()
+    params = [*proj.parameters()]
+    leaves = [m.requires_grad_(True) for m in maps]
+    got = torch.autograd.grad(proj(leaves)[0], [*params, *leaves], dy)
+    twin = LevelInputProjection([24, 40], 64, 16).double().cuda()
+    twin.load_state_dict(proj.state_dict())
+    wide = [m.detach().double().requires_grad_(True) for m in maps]
+    out = flatten_levels([
+        torch.nn.functional.silu(torch.nn.functional.group_norm(
+            torch.nn.functional.conv2d(m, p.weight[:, :, None, None], p.bias), 16, twin.norm_weight[i],
+            twin.norm_bias[i]))
+        for i, (m, p) in enumerate(zip(wide, twin.projections))])[0]
+    want = torch.autograd.grad(out, [*twin.parameters(), *wide], dy.double())
+    for a, b in zip(got, want):
+        # fp32 GEMMs over up to 34816 tokens; a bias before a norm has a gradient of rounding alone
+        assert (a - b).norm() <= 1e-4 * b.norm() + 1e-2
+
+
 def test_masks_of_a_state_from_torchs_generator():
     a = new_rng_state("cuda", torch.Generator(device="cuda").manual_seed(3))
     b = new_rng_state("cuda", torch.Generator(device="cuda").manual_seed(3))

@@ -11,6 +11,10 @@
 // thread keeps its channels for the whole chunk and sums per channel in registers; groups are formed
 // from channels once per chunk.  The passes that write take short chunks (a workgroup a few rows a
 // thread, all their loads in flight at once), which need the level's joined sums and not its chunks'.
+//
+// Bound by HBM, which every tensor but the last crosses twice a direction (MI355X, 8 x 43008 rows of
+// 256 fp32 channels, 352 MB a tensor): sums 56 us, 6.3 TB/s; forward pass 112 us, 6.3 TB/s; sums of
+// the gradient 113 us, 6.2 TB/s; its pass 162 us, 6.5 TB/s; the joins 5 and 6 us.
 #pragma once
 
 #include "msda_vec.h"
@@ -55,8 +59,8 @@ __device__ __forceinline__ int gn_lane_rows(int rows, int r, int lanes) {
   return r < rows ? (rows - r + lanes - 1) / lanes : 0;
 }
 
-// Calls f(Pack (&)[K], rows r0, r0 + lanes, ...) for the thread's rows with the loads of
-// kGnRowsAhead rows issued before the first is used.  `load` fills one row's packs.
+// Calls load(p, r) and use(p, r) for the thread's rows r0, r0 + lanes, ... of a chunk, the loads of
+// kGnRowsAhead rows issued before the first is used.
 template <typename P, typename Load, typename Use>
 __device__ __forceinline__ void gn_rows(int r0, int rows, int lanes, Load load, Use use) {
   constexpr int U = kGnRowsAhead;
