@@ -675,6 +675,20 @@ def test_group_norm_widest_rows(dtype, c, groups):
         del PYRAMIDS["_widest"]
 
 
+@pytest.mark.parametrize("dtype,c,groups,full", [
+    (F32, 256, 1, 64), (F32, 256, 2, 128), (BF16, 256, 1, 128), (BF16, 256, 32, 1024), (F32, 256, 32, 1024),
+    (F16, 64, 2, 1024), (F32, 48, 2, 340), (BF16, 96, 32, 340), (F32, 4, 1, 4096), (BF16, 8, 2, 4096)])
+@pytest.mark.parametrize("extra", [0, 1])
+def test_group_norm_full_workgroups(dtype, c, groups, full, extra):
+    """Levels of as many rows as a workgroup of 1024 threads holds (four vectors a thread), and of one
+    row more, beside a level of half and one of a single row."""
+    PYRAMIDS["_full"] = (2, [(1, full + extra), (1, full // 2), (1, 1)], c, groups)
+    try:
+        run_group("_full", dtype, F32, "silu")
+    finally:
+        del PYRAMIDS["_full"]
+
+
 def test_group_norm_many_samples():
     """More (sample, level) pairs than rows in each, through the one-launch and the general kernels."""
     for n, levels, c, groups in ((5000, [(1, 2), (1, 1)], 16, 4), (3000, [(1, 3)], 6, 3), (4000, [(4, 4)], 256, 32)):

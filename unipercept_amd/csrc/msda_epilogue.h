@@ -400,14 +400,15 @@ int gn_backward(const GnCall& a, const GnPlan& plan) {
 }
 
 // A slab of whole groups for the one-launch kernels, and the threads of its workgroup; false where a
-// level does not fit or the call is too large for slabs of 64 bytes a row (they use half of each
-// cache line).  One launch against three (MI355X, 256 bf16 channels, forward and backward, us):
-// 512 rows 9.9 + 10.3 against 11.2 + 12.6, 64 x 256 rows 10.6 + 16.0 against 13.9 + 17.9; with four
-// vectors a thread it loses (8 x 1024 rows 11.7 + 16.9 against 12.0 + 14.3), so does a slab of 32
-// bytes (17.5 for the latter), and so do 128 x 1024 rows of 512 channels (118 + 184 against 74 + 130).
+// level does not fit `hold` vectors a thread or the call is too large for slabs of 64 bytes a row (they
+// use half of each cache line).  One launch against three (MI355X, 256 bf16 channels, us): forward 512
+// rows 6.9 against 11.2, 64 x 256 rows 8.0 / 13.9, 8 x 1024 rows (four vectors a thread) 8.7 / 11.7;
+// gradient 512 rows 10.3 / 12.6, 64 x 256 rows 16.0 / 17.9.  The gradient with four vectors a thread
+// loses (8 x 1024 rows 16.9 / 14.3), so does a slab of 32 bytes (17.5 for the latter), and so do
+// 128 x 1024 rows of 512 channels (118 + 184 / 74 + 130).
 constexpr int64_t kGnSmallBytes = 16 << 20;
-inline bool gn_small_plan(const GnPlan& plan, int N, int C, int G, size_t esize, GnSlab* sl,
-                          int* threads) {
+inline bool gn_small_plan(const GnPlan& plan, int N, int C, int G, size_t esize, int hold,
+                          GnSlab* sl, int* threads) {
   const int VE = 16 / static_cast<int>(esize), cpg = C / G, S = plan.sums.row_start[plan.sums.levels];
   if (static_cast<int64_t>(N) * S * C * static_cast<int64_t>(esize) > kGnSmallBytes) return false;
   int longest = 0;
@@ -420,13 +421,13 @@ inline bool gn_small_plan(const GnPlan& plan, int N, int C, int G, size_t esize,
     const int vecs = k * cpg / VE;
     if (G % k == 0 && k * cpg % VE == 0 && (vecs >= 4 || k == G)) best = k;
   }
-  if (best == 0 || longest > 1024 / (best * cpg / VE) * kGnHold ||
+  if (best == 0 || longest > 1024 / (best * cpg / VE) * hold ||
       static_cast<int64_t>(N) * plan.sums.levels * (G / best) > (1 << 21))
     return false;
   *sl = {best, best * cpg, best * cpg / VE, G / best};
   *threads = 1024;
   for (int t = 256; t < 1024; t *= 2)
-    if (longest <= t / sl->vecs * kGnHold) {
+    if (longest <= t / sl->vecs * 2) {  // (two vectors a thread: more rows a thread were no faster)
       *threads = t;
       break;
     }
@@ -483,7 +484,8 @@ int gn_act_run(const GnCall& a, const GnPlan& plan, bool backward) {
   if constexpr (sizeof(T) <= 4) {
     GnSlab sl;
     int threads;
-    if (gn_small_plan(plan, a.N, a.C, a.G, sizeof(T), &sl, &threads))
+    if (gn_small_plan(plan, a.N, a.C, a.G, sizeof(T), backward ? kGnHoldBwd : kGnHold, &sl,
+                      &threads))
       return backward ? gn_small_backward<T, ACT>(a, plan, sl, threads)
                       : gn_small_forward<T, ACT>(a, plan, sl, threads);
   }
