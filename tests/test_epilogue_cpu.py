@@ -231,6 +231,67 @@ def test_gradients_have_shapes_without_running():
     assert [g.shape for g in grads] == [t.shape for t in (x, res, w, b)]
 
 
+def _calls_by_input():
+    """(operator, input) -> a function of that input alone, on the meta device."""
+    big, one = (2, 20, 8), (8,)
+    drop = lambda x, act: counter_dropout(x, 0.0 if act == "relu" else 0.1, STATE, 1, act)
+    norm = lambda **kw: dropout_add_layer_norm(
+        **{**dict(x=meta(*big), residual=meta(*big), weight=meta(*one), bias=meta(*one)), **kw})
+    group = lambda **kw: level_group_norm(
+        **{**dict(x=meta(*big), weight=meta(*one), bias=meta(*one), num_groups=4), **kw})
+    calls = {("dropout", act): (big, lambda t, act=act: drop(t, act)) for act in ("none", "relu")}
+    for name in ("x", "residual", "weight", "bias"):
+        shape = big if name in ("x", "residual") else one
+        calls["norm", name] = (shape, lambda t, name=name: norm(**{name: t}))
+        if name != "residual":
+            calls["group", name] = (shape, lambda t, name=name: group(**{name: t}))
+    return calls
+
+
+@pytest.mark.parametrize("call", sorted(_calls_by_input()))
+def test_forward_mode_derivatives_are_refused(call):
+    """A tangent on any input raises, whether or not the input requires a gradient as well: an output
+    without a tangent would count as a derivative of zero."""
+    from torch.autograd import forward_ad
+
+    shape, f = _calls_by_input()[call]
+    for requires_grad in (False, True):
+        with forward_ad.dual_level():
+            t = forward_ad.make_dual(meta(*shape).requires_grad_(requires_grad), meta(*shape))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                f(t)
+            with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+                f(t)
+    with pytest.raises(NotImplementedError, match="forward-mode"):
+        torch.func.jvp(f, (meta(*shape),), (meta(*shape),))
+    # without a tangent, inside a dual level, everything runs
+    with forward_ad.dual_level():
+        f(meta(*shape))
+
+
+@pytest.mark.parametrize("call", sorted(_calls_by_input()))
+def test_a_tangent_of_the_incoming_gradient_is_refused(call):
+    from torch.autograd import forward_ad
+
+    shape, f = _calls_by_input()[call]
+    t = meta(*shape).requires_grad_(True)
+    y = f(t)
+    with forward_ad.dual_level():
+        dy = forward_ad.make_dual(meta(*y.shape), meta(*y.shape))
+        for create_graph in (False, True):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, t, dy, retain_graph=True, create_graph=create_graph)
+    assert torch.autograd.grad(y, t, meta(*y.shape))[0].shape == shape
+
+
+def test_dropout_of_nothing_keeps_its_tangent():
+    from torch.autograd import forward_ad
+
+    with forward_ad.dual_level():
+        t = forward_ad.make_dual(meta(4), meta(4))
+        assert forward_ad.unpack_dual(counter_dropout(t, 0.0)).tangent is not None
+
+
 def test_torch_operators_are_built_and_loud_when_missing(monkeypatch, tmp_path):
     assert _lib.torch_ops() is torch.ops.unipercept
     monkeypatch.setattr(_lib, "_torch_ops", None)

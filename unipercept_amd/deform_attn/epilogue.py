@@ -7,8 +7,8 @@
   activation.
 
 All take float32, float64, bfloat16 and float16 tensors on a ROCm GPU (sums and statistics are held
-in 32 bits or more), use the current stream, are differentiable once, and give the same bits on every
-run.  ``MSDeformAttnEncoderLayer(fused_epilogues=True)`` and ``LevelInputProjection`` call them.
+in 32 bits or more), use the current stream, are differentiable once in reverse mode (a forward-mode
+tangent raises ``NotImplementedError``), and give the same bits on every run.  ``MSDeformAttnEncoderLayer(fused_epilogues=True)`` and ``LevelInputProjection`` call them.
 """
 
 from __future__ import annotations

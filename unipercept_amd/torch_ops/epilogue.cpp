@@ -446,6 +446,14 @@ struct BelowAutograd {
   }
 };
 
+// The operators have no forward-mode derivatives: a tangent would be dropped without a word below
+// autograd, and a missing tangent counts as zero.
+void refuse_tangents(const char* what, std::initializer_list<const Tensor*> tensors) {
+  for (const Tensor* t : tensors)
+    TORCH_CHECK_NOT_IMPLEMENTED(!t->_fw_grad(/*level=*/0).defined(), what,
+                                ": forward-mode derivatives are not implemented");
+}
+
 OptTensor optional_of(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 struct DropoutNode : torch::autograd::Function<DropoutNode> {
@@ -462,6 +470,7 @@ struct DropoutNode : torch::autograd::Function<DropoutNode> {
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
+    refuse_tangents(kDrop, {&grads[0]});
     BelowAutograd below;
     Tensor gx = call_dropout_bwd(grads[0], optional_of(saved[0]), optional_of(saved[1]),
                                  ctx->saved_data["p"].toDouble(), ctx->saved_data["site"].toInt(),
@@ -491,6 +500,7 @@ struct AddNormNode : torch::autograd::Function<AddNormNode> {
     const bool need_w = ctx->needs_input_grad(2), need_b = ctx->needs_input_grad(3);
     // nothing dropped and one type: both gradients are the same tensor
     const bool shared = p == 0.0 && saved[0].scalar_type() == saved[1].scalar_type();
+    refuse_tangents(kNorm, {&grads[0]});
     BelowAutograd below;
     Tensor gx, gr, gw, gb;
     std::tie(gx, gr, gw, gb) =
@@ -520,6 +530,7 @@ struct GroupNormNode : torch::autograd::Function<GroupNormNode> {
     const variable_list saved = ctx->get_saved_variables();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
     const bool need_b = ctx->needs_input_grad(2);
+    refuse_tangents(kGroup, {&grads[0]});
     BelowAutograd below;
     Tensor gx, gw, gb;
     std::tie(gx, gw, gb) = op.call(
@@ -546,6 +557,7 @@ Tensor counter_dropout(const Tensor& x, double p, const OptTensor& state_, int64
   activation_code(kDrop, activation, true);
   check_rng(kDrop, p, site, given(state_), x);
   if (p == 0.0 && activation == "none") return x;
+  refuse_tangents(kDrop, {&x});
   const OptTensor state = p > 0.0 ? state_ : OptTensor();
   if (grad_wanted({&x})) return DropoutNode::apply(x, state, p, site, activation);
   BelowAutograd below(true);
@@ -556,6 +568,7 @@ Tensor dropout_add_layer_norm(const Tensor& x, const Tensor& residual, const Ten
                               const Tensor& bias, double p, const OptTensor& state_, int64_t site,
                               double eps) {
   check_add_norm(x, residual, weight, bias, given(state_), p, site, eps);
+  refuse_tangents(kNorm, {&x, &residual, &weight, &bias});
   const OptTensor state = p > 0.0 ? state_ : OptTensor();
   if (grad_wanted({&x, &residual, &weight, &bias}))
     return AddNormNode::apply(x, residual, weight, bias, state, p, site, eps);
@@ -569,6 +582,7 @@ Tensor level_group_norm(const Tensor& x, const Tensor& weight, const Tensor& bia
   activation_code(kGroup, activation, false);
   const std::vector<int64_t> rows = level_rows(x, rows_);
   check_group_norm(x, weight, bias, groups, rows, eps);
+  refuse_tangents(kGroup, {&x, &weight, &bias});
   if (grad_wanted({&x, &weight, &bias}))
     return GroupNormNode::apply(x, weight, bias, groups, IntArrayRef(rows), eps, activation);
   BelowAutograd below(true);
