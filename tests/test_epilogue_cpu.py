@@ -292,6 +292,36 @@ def test_dropout_of_nothing_keeps_its_tangent():
         assert forward_ad.unpack_dual(counter_dropout(t, 0.0)).tangent is not None
 
 
+@pytest.mark.parametrize("name", ["dropout", "norm"])
+def test_vmap_does_not_repeat_a_mask_unasked(name):
+    """Samples of a vmap count their elements from 0 each: refused unless the caller asks for equal
+    masks or maps the states with the samples."""
+    w = meta(8)
+    f = {"dropout": lambda x, state, p=0.1: counter_dropout(x, p, state, 1, "relu"),
+         "norm": lambda x, state, p=0.1: dropout_add_layer_norm(x, x, w, w, p, state)}[name]
+    x, states = meta(3, 5, 8), meta(3, 2, dtype=torch.int64)
+    vmap = torch.func.vmap
+    for mode in ("error", "different"):
+        refused = "randomness error mode" if mode == "error" else "same mask"
+        with pytest.raises(RuntimeError, match=refused):
+            vmap(lambda t: f(t, STATE), randomness=mode)(x)
+        assert vmap(f, randomness=mode)(x, states).shape == x.shape
+        assert vmap(lambda t: f(t, STATE, 0.0), randomness=mode)(x).shape == x.shape
+        # an outer map without states of its own
+        with pytest.raises(RuntimeError, match=refused):
+            vmap(lambda a: vmap(f, randomness=mode)(a, states), randomness=mode)(meta(4, 3, 5, 8))
+        both = vmap(vmap(f, randomness=mode), randomness=mode)
+        assert both(meta(4, 3, 5, 8), meta(4, 3, 2, dtype=torch.int64)).shape == (4, 3, 5, 8)
+    assert vmap(lambda t: f(t, STATE), randomness="same")(x).shape == x.shape
+    outer = meta(3, 5, 8).requires_grad_(True)
+    y = vmap(lambda t: f(t, STATE), randomness="same")(outer)
+    assert torch.autograd.grad(y, outer, meta(3, 5, 8))[0].shape == x.shape
+    # gradients of a batch of incoming gradients: one forward, one mask
+    leaf = meta(5, 8).requires_grad_(True)
+    y = f(leaf, STATE)
+    assert torch.autograd.grad(y, leaf, meta(3, 5, 8), is_grads_batched=True)[0].shape == (3, 5, 8)
+
+
 def test_torch_operators_are_built_and_loud_when_missing(monkeypatch, tmp_path):
     assert _lib.torch_ops() is torch.ops.unipercept
     monkeypatch.setattr(_lib, "_torch_ops", None)

@@ -8,7 +8,8 @@
 
 All take float32, float64, bfloat16 and float16 tensors on a ROCm GPU (sums and statistics are held
 in 32 bits or more), use the current stream, are differentiable once in reverse mode (a forward-mode
-tangent raises ``NotImplementedError``), and give the same bits on every run.  ``MSDeformAttnEncoderLayer(fused_epilogues=True)`` and ``LevelInputProjection`` call them.
+tangent raises ``NotImplementedError``), and give the same bits on every run.
+``MSDeformAttnEncoderLayer(fused_epilogues=True)`` and ``LevelInputProjection`` call them.
 """
 
 from __future__ import annotations
@@ -57,7 +58,11 @@ def counter_dropout(
     the scale belongs to that value.  A dropped element is 0 whatever x holds.  The state is read when
     the kernel runs, so a captured graph draws new masks if the caller changes it between replays;
     do not change it between a forward and its backward.  Without anything to do (p = 0, no
-    activation) x itself is returned."""
+    activation) x itself is returned.
+
+    Under ``torch.func.vmap`` every sample counts its own elements from 0 and would drop the same ones:
+    that is what ``randomness="same"`` asks for; with another mode the call is refused unless the
+    states are mapped with the samples.  A call on the whole batch draws a mask for all of it."""
     return _lib.torch_ops().counter_dropout(x, p, rng_state, site, activation)
 
 

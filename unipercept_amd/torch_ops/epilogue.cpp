@@ -13,12 +13,14 @@
 //
 // libmsda.so is loaded, with its symbols global, before this library.
 #include <ATen/ATen.h>
+#include <ATen/functorch/BatchedTensorImpl.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -589,10 +591,61 @@ Tensor level_group_norm(const Tensor& x, const Tensor& weight, const Tensor& bia
   return std::get<0>(call_group_norm_fwd(x, weight, bias, groups, rows, eps, activation, false));
 }
 
+// ---- vmap ---------------------------------------------------------------------------------------------
+
+// Levels of torch.func.vmap that a tensor is mapped at.
+std::vector<int64_t> mapped_levels(const Tensor& t) {
+  std::vector<int64_t> levels;
+  const at::functorch::BatchedTensorImpl* batched = at::functorch::maybeGetBatchedImpl(t);
+  for (; batched != nullptr; batched = at::functorch::maybeGetBatchedImpl(batched->value()))
+    levels.push_back(batched->level());
+  return levels;
+}
+
+// vmap runs an operator sample by sample, each from element 0 of the same state: every sample would
+// drop the same elements.  Right where the caller asks for that (randomness "same") or maps the states
+// with the samples; refused otherwise.
+void check_vmap(const char* what, double p, const Tensor& state, std::initializer_list<const Tensor*> tensors) {
+  if (p == 0.0) return;
+  std::vector<int64_t> repeated;
+  for (const Tensor* t : tensors)
+    for (int64_t level : mapped_levels(*t)) repeated.push_back(level);
+  if (repeated.empty()) return;
+  for (int64_t level : mapped_levels(state))
+    repeated.erase(std::remove(repeated.begin(), repeated.end(), level), repeated.end());
+  if (repeated.empty()) return;
+  // torch's own random operators know the mode: no numbers at all are drawn here, which raises in mode
+  // "error" and returns a mapped tensor in mode "different"
+  for (int64_t level : mapped_levels(at::rand({0}, at::TensorOptions(at::kCPU))))
+    TORCH_CHECK(std::find(repeated.begin(), repeated.end(), level) == repeated.end(), what,
+                ": every sample of this vmap would get the same mask; map rng_state with the samples, or "
+                "call the operator on the batch");
+}
+
+// Under vmap: checked, then sample by sample (the *_each operators have no kernel here).
+Tensor counter_dropout_vmap(const Tensor& x, double p, const OptTensor& state, int64_t site,
+                            const std::string& activation) {
+  check_vmap(kDrop, p, given(state), {&x});
+  static const auto op = find<decltype(counter_dropout)>("unipercept::counter_dropout_each");
+  return op.call(x, p, state, site, activation);
+}
+
+Tensor dropout_add_layer_norm_vmap(const Tensor& x, const Tensor& residual, const Tensor& weight,
+                                   const Tensor& bias, double p, const OptTensor& state, int64_t site,
+                                   double eps) {
+  check_vmap(kNorm, p, given(state), {&x, &residual, &weight, &bias});
+  static const auto op = find<decltype(dropout_add_layer_norm)>("unipercept::dropout_add_layer_norm_each");
+  return op.call(x, residual, weight, bias, p, state, site, eps);
+}
+
 }  // namespace
 
 TORCH_LIBRARY_FRAGMENT(unipercept, m) {
   m.def("counter_dropout(Tensor x, float p, Tensor? rng_state, int site, str activation) -> Tensor");
+  m.def("counter_dropout_each(Tensor x, float p, Tensor? rng_state, int site, str activation) -> Tensor");
+  m.def(
+      "dropout_add_layer_norm_each(Tensor x, Tensor residual, Tensor weight, Tensor bias, float p, "
+      "Tensor? rng_state, int site, float eps) -> Tensor");
   m.def("counter_dropout_fwd(Tensor x, Tensor? rng_state, float p, int site, str activation) -> Tensor");
   m.def(
       "counter_dropout_bwd(Tensor grad_output, Tensor? out, Tensor? rng_state, float p, int site, "
@@ -623,6 +676,13 @@ TORCH_LIBRARY_IMPL(unipercept, CompositeImplicitAutograd, m) {
   m.impl("counter_dropout", counter_dropout);
   m.impl("dropout_add_layer_norm", dropout_add_layer_norm);
   m.impl("level_group_norm", level_group_norm);
+  m.impl("counter_dropout_each", counter_dropout);
+  m.impl("dropout_add_layer_norm_each", dropout_add_layer_norm);
+}
+
+TORCH_LIBRARY_IMPL(unipercept, FuncTorchBatched, m) {
+  m.impl("counter_dropout", counter_dropout_vmap);
+  m.impl("dropout_add_layer_norm", dropout_add_layer_norm_vmap);
 }
 
 TORCH_LIBRARY_IMPL(unipercept, CUDA, m) {
