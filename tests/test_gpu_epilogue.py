@@ -428,6 +428,54 @@ def test_group_norm_outliers_and_not_finite_groups():
     assert torch.equal(const, torch.full_like(const, 0.25))
 
 
+GATE = {
+    # (samples, levels, channels, groups): one launch, whole vectors and parts of vectors a group
+    "small": (2, [(8, 16), (4, 8)], 64, 8),
+    "small_parts": (2, [(8, 16), (4, 8)], 64, 32),
+    # the forward in one launch, the gradient in three
+    "mixed": (2, [(1, 1024), (1, 3)], 256, 32),
+    "long": (2, [(96, 130), (1, 9)], 64, 8),
+    "long_odd": (1, [(96, 130), (2, 9)], 21, 3),
+    "long_short": (1, [(130, 130)], 3, 3),
+}
+
+
+@pytest.mark.parametrize("case", sorted(GATE))
+@pytest.mark.parametrize("dtype", [F32, BF16, F64])
+def test_group_norm_relu_gate_is_one_in_every_pass(case, dtype):
+    """Elements whose z is a rounding away from 0: what the output shows as open is open in dx, dw and
+    db, in every kernel.  Given the gate the gradient is that of the plain norm for the gated incoming
+    gradient, with its bounds."""
+    n, levels, c, groups = GATE[case]
+    rows = [h * w for h, w in levels]
+    wide = F64 if dtype == F64 else F32
+    g = torch.Generator().manual_seed(len(case))
+    x = (torch.randint(-8, 9, (n, sum(rows), c), generator=g).double() * 0.25 + 0.375).to(dtype)  # few values
+    w = normal((len(rows), c), wide, 5, 0.3, 1.0)
+    zero = torch.zeros_like(w)
+    _, mean, rstd = _lib.torch_ops().level_group_norm_fwd(
+        x.cuda(), w.cuda(), zero.cuda(), groups, rows, 1e-5, "relu", True)
+    mean, rstd = (t.cpu().repeat_interleave(c // groups, -1) for t in (mean, rstd))  # (n, L, c)
+    b, start = torch.empty_like(w), 0
+    for level, r in enumerate(rows):
+        # z = 0 but for its rounding where a channel has the value of its first row of the first sample
+        b[level] = -(x[0, start].to(wide) - mean[0, level]) * (rstd[0, level] * w[level])
+        start += r
+    leaves = [t.cuda().requires_grad_(True) for t in (x, w, b)]
+    out = level_group_norm(*leaves, groups, levels, 1e-5, "relu")
+    out.backward(torch.ones_like(out))
+    opened = out.detach().cpu() > 0
+    dz = opened.to(dtype)
+    _, parts = ref.group_norm(x, w, b, groups, rows, 1e-5, "none")
+    z = torch.cat([q["z"] for q in parts], 1)
+    assert (z.abs() < 1e-5).any(1).any(0).sum() > c // 2  # the case holds what it is about
+    bounds = group_bounds(x, parts, dz, "none", dtype)[1:]
+    assert torch.equal(leaves[2].grad.cpu().double(), torch.stack(
+        [v.double().sum((0, 1)) for v in dz.split(rows, 1)]))  # whole numbers
+    for name, t, want, bound in zip(("dx", "dw"), leaves, ref.group_norm_grad(dz, parts, "none"), bounds):
+        check((name, case, dtype), t.grad, want, bound + half_step(want, t.grad.dtype))
+
+
 def test_group_norm_empty_and_partial_gradients():
     w, b = torch.ones(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda", requires_grad=True)
     for shape in ((0, 5, 8), (3, 0, 8)):

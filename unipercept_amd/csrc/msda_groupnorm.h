@@ -166,6 +166,25 @@ __device__ __forceinline__ CT gn_slope(CT z) {
   return CT(1);
 }
 
+// ---- the normalised value ---------------------------------------------------------------------------
+// z = (x - mean) * (rstd * weight) + bias decides the ReLU's gate, and an element whose z is a rounding
+// away from 0 has to be open in all of y, dx, dw and db or in none.  So every pass of both directions
+// forms z and what it is made of by these functions alone, whose roundings the compiler may not change.
+template <typename CT>
+__device__ __forceinline__ CT gn_times(CT a, CT b) {
+#pragma clang fp contract(off)
+  return a * b;
+}
+template <typename CT>
+__device__ __forceinline__ CT gn_centred(CT x, CT mean) {
+#pragma clang fp contract(off)
+  return x - mean;
+}
+__device__ __forceinline__ float gn_affine(float d, float scale, float bias) { return fmaf(d, scale, bias); }
+__device__ __forceinline__ double gn_affine(double d, double scale, double bias) { return fma(d, scale, bias); }
+// 1 / sqrt(sum / count + eps), inv = 1 / count
+__device__ __forceinline__ float gn_rstd(float sum, float inv, float eps) { return 1.f / sqrtf(fmaf(sum, inv, eps)); }
+
 // ---- forward ----------------------------------------------------------------------------------------
 // partial[(block * G + g) * 2] = (mean, M2) of the chunk's rows of group g.
 // Thread-level sums are taken about the first value that the thread reads of each channel, so a
@@ -347,7 +366,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(
   load_params<T>(weight, pl, sp, wide != 0, w);
   load_params<T>(bias, pl, sp, wide != 0, b);
 #pragma unroll
-  for (int i = 0; i < VE; ++i) a[i] *= w[i];
+  for (int i = 0; i < VE; ++i) a[i] = gn_times(a[i], w[i]);
   const T* src = x + ch.first_row * C;
   T* dst = out + ch.first_row * C;
   gn_rows<P>(
@@ -356,7 +375,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_apply_kernel(
         ct v[VE];
         p.unpack(v);
 #pragma unroll
-        for (int i = 0; i < VE; ++i) v[i] = gn_act<ACT>((v[i] - mu[i]) * a[i] + b[i]);
+        for (int i = 0; i < VE; ++i) v[i] = gn_act<ACT>(gn_affine(gn_centred(v[i], mu[i]), a[i], b[i]));
         p.pack(v);
         sp.store(p, dst + static_cast<int64_t>(r) * C);
       });
@@ -404,7 +423,7 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(
     }
 #pragma unroll
     for (int i = 0; i < VE; ++i) {
-      a[i] *= s[i];
+      a[i] = gn_times(s[i], a[i]);
       dw[i] = db[i] = 0;
     }
     gn_rows<P>(
@@ -419,9 +438,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_stats_kernel(
           p.g.unpack(gv);
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            const ct d = xv[i] - mu[i];
+            const ct d = gn_centred(xv[i], mu[i]);
             ct dz = gv[i];
-            if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(d * a[i] + b[i]);
+            if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(gn_affine(d, a[i], b[i]));
             dw[i] += dz * d;
             db[i] += dz;
           }
@@ -524,13 +543,15 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(
   const auto sp = Span<VE, MODE>::at(k, C);
   const int64_t pl = param_levels > 1 ? static_cast<int64_t>(ch.level) * C : 0;
   const int64_t sg = (static_cast<int64_t>(ch.n) * cut.levels + ch.level) * G;
-  ct mu[VE], s[VE], w[VE], b[VE], a1[VE], a2[VE];
+  ct mu[VE], s[VE], w[VE], b[VE], sw[VE], a1[VE], a2[VE];
   gn_spread(mean + sg, sp, cpg, mu);
   gn_spread(rstd + sg, sp, cpg, s);
   gn_spread(m1 + sg, sp, cpg, a1);
   gn_spread(m2 + sg, sp, cpg, a2);
   load_params<T>(weight, pl, sp, wide != 0, w);
   if constexpr (ACT != kGnNone) load_params<T>(bias, pl, sp, wide != 0, b);
+#pragma unroll
+  for (int i = 0; i < VE; ++i) sw[i] = gn_times(s[i], w[i]);
   const T* sx = x + ch.first_row * C;
   const T* sd = grad_out + ch.first_row * C;
   T* dst = grad_x + ch.first_row * C;
@@ -546,9 +567,9 @@ __global__ __launch_bounds__(kGnThreads) void gn_bwd_apply_kernel(
         p.g.unpack(gv);
 #pragma unroll
         for (int i = 0; i < VE; ++i) {
-          const ct u = (xv[i] - mu[i]) * s[i];
+          const ct d = gn_centred(xv[i], mu[i]), u = d * s[i];
           ct dz = gv[i];
-          if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[i] + b[i]);
+          if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(gn_affine(d, sw[i], b[i]));
           gv[i] = s[i] * (w[i] * dz - a1[i] - u * a2[i]);
         }
         p.g.pack(gv);
@@ -693,14 +714,14 @@ __global__ __launch_bounds__(1024) void gn_small_kernel(
     float t = 0;
 #pragma unroll
     for (int e = 0; e < VE; ++e) t += sum[e];
-    t = gn_small_sum_whole(t, m, sl, lds) * inv;
+    t = gn_times(gn_small_sum_whole(t, m, sl, lds), inv);
 #pragma unroll
     for (int e = 0; e < VE; ++e) mu[e] = t;
   } else {
     gn_small_sum<VE>(sum, s, sl, cpg, lds, totals);
     gn_spread(totals, sp, cpg, mu);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) mu[e] *= inv;
+    for (int e = 0; e < VE; ++e) mu[e] = gn_times(mu[e], inv);
   }
 #pragma unroll
   for (int e = 0; e < VE; ++e) sum[e] = 0;
@@ -719,7 +740,7 @@ __global__ __launch_bounds__(1024) void gn_small_kernel(
     for (int e = 0; e < VE; ++e) t += sum[e];
     // (behind the first sum's values, which other waves may still read; 2 * waves * vecs <= lanes *
     // channels, as a slab has vecs <= 64 and four channels or more a vector)
-    t = 1.f / sqrtf(gn_small_sum_whole(t, m, sl, lds + (blockDim.x >> 6) * sl.vecs) * inv + eps);
+    t = gn_rstd(gn_small_sum_whole(t, m, sl, lds + (blockDim.x >> 6) * sl.vecs), inv, eps);
 #pragma unroll
     for (int e = 0; e < VE; ++e) a[e] = t;
     const int kv = sp.c / VE;
@@ -731,22 +752,22 @@ __global__ __launch_bounds__(1024) void gn_small_kernel(
     gn_small_sum<VE>(sum, s, sl, cpg, lds, squares);
     if (mean != nullptr)
       for (int g = threadIdx.x; g < sl.groups; g += blockDim.x) {
-        mean[cell + g] = totals[g] * inv;
-        rstd[cell + g] = 1.f / sqrtf(squares[g] * inv + eps);
+        mean[cell + g] = gn_times(totals[g], inv);
+        rstd[cell + g] = gn_rstd(squares[g], inv, eps);
       }
     gn_spread(squares, sp, cpg, a);
 #pragma unroll
-    for (int e = 0; e < VE; ++e) a[e] = 1.f / sqrtf(a[e] * inv + eps);
+    for (int e = 0; e < VE; ++e) a[e] = gn_rstd(a[e], inv, eps);
   }
 #pragma unroll
-  for (int e = 0; e < VE; ++e) a[e] *= w[e];
+  for (int e = 0; e < VE; ++e) a[e] = gn_times(a[e], w[e]);
 #pragma unroll
   for (int i = 0; i < kGnHold; ++i)
     if (i < s.count) {
       float v[VE];
       p[i].unpack(v);
 #pragma unroll
-      for (int e = 0; e < VE; ++e) v[e] = gn_act<ACT>((v[e] - mu[e]) * a[e] + b[e]);
+      for (int e = 0; e < VE; ++e) v[e] = gn_act<ACT>(gn_affine(gn_centred(v[e], mu[e]), a[e], b[e]));
       p[i].pack(v);
       p[i].template store<false>(out + s.base + i * step);
     }
@@ -779,13 +800,16 @@ __global__ __launch_bounds__(1024) void gn_small_bwd_kernel(
   const Span<VE, kRowEven> sp = {c0, 0, VE};
   const int64_t cell = (static_cast<int64_t>(s.n) * cut.levels + s.level) * G + s.slab * sl.groups;
   const int64_t pc = (param_levels > 1 ? static_cast<int64_t>(s.level) * C : 0) + s.slab * sl.channels;
-  float mu[VE], r[VE], w[VE], b[VE], sums[2][VE];
+  float mu[VE], r[VE], w[VE], b[VE], rw[VE], sums[2][VE];
   gn_spread(mean + cell, sp, cpg, mu);
   gn_spread(rstd + cell, sp, cpg, r);
   load_params<T>(weight, pc, sp, wide != 0, w);
   load_params<T>(bias, pc, sp, wide != 0, b);
 #pragma unroll
-  for (int e = 0; e < VE; ++e) sums[0][e] = sums[1][e] = 0;
+  for (int e = 0; e < VE; ++e) {
+    rw[e] = gn_times(r[e], w[e]);
+    sums[0][e] = sums[1][e] = 0;
+  }
 #pragma unroll
   for (int i = 0; i < HOLD; ++i)
     if (i < s.count) {
@@ -794,9 +818,9 @@ __global__ __launch_bounds__(1024) void gn_small_bwd_kernel(
       pg[i].unpack(gv);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float u = (xv[e] - mu[e]) * r[e];
+        const float d = gn_centred(xv[e], mu[e]), u = d * r[e];
         float dz = gv[e];
-        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[e] + b[e]);
+        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(gn_affine(d, rw[e], b[e]));
         sums[0][e] += dz * u;
         sums[1][e] += dz;
       }
@@ -847,9 +871,9 @@ __global__ __launch_bounds__(1024) void gn_small_bwd_kernel(
       pg[i].unpack(gv);
 #pragma unroll
       for (int e = 0; e < VE; ++e) {
-        const float u = (xv[e] - mu[e]) * r[e];
+        const float d = gn_centred(xv[e], mu[e]), u = d * r[e];
         float dz = gv[e];
-        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(u * w[e] + b[e]);
+        if constexpr (ACT != kGnNone) dz *= gn_slope<ACT>(gn_affine(d, rw[e], b[e]));
         gv[e] = r[e] * (w[e] * dz - m1[e] - u * m2[e]);
       }
       pg[i].pack(gv);
