@@ -463,6 +463,58 @@ def test_encoder_passes_its_old_arguments_to_foreign_layers():
     src, shapes, lsi, levels, _ = flatten_levels([torch.zeros(1, 16, 2, 3)])
     assert torch.equal(enc(src, shapes, lsi, spatial_shapes_list=levels), src + 1)
 
+def _watched(monkeypatch):
+    """The fused route's operators replaced by recorders: (p, whether a state was given) of every call."""
+    from unipercept_amd.deform_attn import encoder
+
+    seen = []
+
+    def norm(x, residual, weight, bias, p=0.0, rng_state=None, site=0, eps=1e-5):
+        seen.append((p, rng_state is not None))
+        return residual
+
+    def drop(x, p, rng_state=None, site=0, activation="none"):
+        seen.append((p, rng_state is not None))
+        return x
+
+    monkeypatch.setattr(encoder, "dropout_add_layer_norm", norm)
+    monkeypatch.setattr(encoder, "counter_dropout", drop)
+    return seen
+
+
+@pytest.mark.parametrize("layer_trains", [False, True])
+@pytest.mark.parametrize("dropout_trains", [False, True])
+def test_fused_dropout_obeys_the_dropout_module(monkeypatch, layer_trains, dropout_trains):
+    """As in the plain route the mode of the dropout module decides, not that of the layer: frozen dropout
+    in a training layer, dropout that stays active in a layer that evaluates."""
+    seen = _watched(monkeypatch)
+    enc = MSDeformAttnEncoder(2, d_model=16, d_ffn=32, dropout=0.25, n_levels=1, n_heads=2, n_points=2,
+                              fused_epilogues=True)
+    src, shapes, lsi, levels, _ = flatten_levels([torch.zeros(1, 16, 2, 3)])
+    for layer in enc.layers:
+        layer.train(layer_trains)
+        layer.dropout.train(dropout_trains)
+        layer.self_attn.forward = lambda query, *args: query
+    want = (0.25, True) if dropout_trains else (0.0, False)
+    enc(src, shapes, lsi, spatial_shapes_list=levels)
+    assert seen == [want] * 6
+    seen.clear()
+    enc.layers[0]._fused_rest(src, src, None, 0)  # a state of its own where one is needed
+    assert seen == [want] * 3
+
+
+def test_fused_route_takes_no_dropout_it_does_not_know(monkeypatch):
+    seen = _watched(monkeypatch)
+    layer = MSDeformAttnEncoderLayer(16, 32, 0.25, n_levels=1, n_heads=2, n_points=2, fused_epilogues=True)
+    src = torch.zeros(1, 6, 16)
+    layer.dropout = torch.nn.Identity()
+    layer._fused_rest(src, src, None, 0)
+    assert seen == [(0.0, False)] * 3
+    for other in (torch.nn.AlphaDropout(0.25), torch.nn.ReLU()):
+        layer.dropout = other
+        with pytest.raises(TypeError, match="nn.Dropout"):
+            layer._fused_rest(src, src, None, 0)
+
 
 def test_fused_routes_refuse_cpu_tensors():
     src, shapes, lsi, levels, _ = flatten_levels([torch.zeros(1, 16, 2, 3)])

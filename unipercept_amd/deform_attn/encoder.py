@@ -85,6 +85,17 @@ def encoder_reference_points(
     return ref[:, :, None, :] * valid_ratios[:, None, :, :]
 
 
+def _dropout_probability(module: nn.Module) -> float:
+    """What the fused route takes from a layer's dropout module: its p while the module itself trains."""
+    if type(module) is nn.Dropout:
+        return module.p if module.training else 0.0
+    if type(module) is nn.Identity:
+        return 0.0
+    raise TypeError(
+        f"fused_epilogues: the layer's dropout must be nn.Dropout or nn.Identity, got {type(module).__name__}"
+    )
+
+
 class MSDeformAttnEncoderLayer(nn.Module):
     """``fused_epilogues``: dropout, the residual sums, the layer norms and the ReLU run in the HIP
     kernels of ``epilogue`` (ROCm tensors only): ``dropout_add_layer_norm`` behind the attention and
@@ -139,7 +150,7 @@ class MSDeformAttnEncoderLayer(nn.Module):
         return self.norm2(src + self.dropout(ffn))
 
     def _fused_rest(self, src, attn, rng_state, rng_site):
-        p = self.dropout.p if self.training else 0.0
+        p = _dropout_probability(self.dropout)
         if p > 0.0 and rng_state is None:
             rng_state = new_rng_state(src.device)
         if torch.is_autocast_enabled("cuda") and src.dtype in (torch.bfloat16, torch.float16):
@@ -185,7 +196,7 @@ class MSDeformAttnEncoder(nn.Module):
         rng_state = None
         for i, layer in enumerate(self.layers):
             args = (src, pos, ref, spatial_shapes, level_start_index, padding_mask)
-            if getattr(layer, "fused_epilogues", False) and layer.training and layer.dropout.p > 0.0:
+            if getattr(layer, "fused_epilogues", False) and _dropout_probability(layer.dropout) > 0.0:
                 if rng_state is None:
                     rng_state = new_rng_state(src.device)
                 args += (rng_state, i * MSDeformAttnEncoderLayer.RNG_SITES)
