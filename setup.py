@@ -63,12 +63,19 @@ class build_hip(Command):
             cmd = hip_command(out)
             print(" ".join(cmd))
             subprocess.run(cmd, check=True)
-        out = ROOT / "unipercept_amd" / "libmsda_torch.so"
-        deps = [*(ROOT / "unipercept_amd" / "torch_ops").glob("*.cpp"), ROOT / "include" / "msda.h"]
-        if not self.force and out.exists() and all(out.stat().st_mtime >= d.stat().st_mtime for d in deps):
-            print(f"{out} is up to date")
+        # always compiled: a library of an earlier build may be another torch's, which its age does not tell
+        try:
+            cmd = torch_ops_command(ROOT / "unipercept_amd" / "libmsda_torch.so")
+        except ModuleNotFoundError as e:
+            if e.name != "torch":
+                raise
+            print(
+                "warning: torch cannot be imported in this build environment, so libmsda_torch.so "
+                "(counter_dropout, dropout_add_layer_norm, level_group_norm) is not built; "
+                "`pip install --no-build-isolation .` builds it against the installed torch",
+                file=sys.stderr,
+            )
             return
-        cmd = torch_ops_command(out)
         print(" ".join(cmd))
         subprocess.run(cmd, check=True)
 

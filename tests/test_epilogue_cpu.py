@@ -345,6 +345,56 @@ def test_packaging_builds_the_same_torch_operators():
     assert entry.build_torch_ops() == out
 
 
+def _packaging(tmp_path, **env):
+    """`setup.py build_hip` in a copy of the sources, the compilers replaced by scripts that write their
+    output file."""
+    import os
+    import shutil
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    import __graft_entry__ as entry
+
+    root, tree = Path(entry.__file__).resolve().parent, tmp_path / "tree"
+    if not tree.exists():
+        for part in ("unipercept_amd/csrc", "unipercept_amd/torch_ops", "include"):
+            shutil.copytree(root / part, tree / part)
+        for part in ("setup.py", "pyproject.toml", "README.md", "unipercept_amd/__init__.py"):
+            shutil.copy(root / part, tree / part)
+    compiler = tmp_path / "compiler"
+    compiler.write_text(
+        "#!/bin/bash\nwhile [ $# -gt 1 ]; do [ \"$1\" = -o ] && echo built >> \"$2\"; shift; done\n")
+    compiler.chmod(0o755)
+    done = subprocess.run(
+        [sys.executable, "setup.py", "build_hip"], cwd=tree, capture_output=True, text=True, timeout=120,
+        env={**os.environ, "HIPCC": str(compiler), "CXX": str(compiler), **env})
+    return tree / "unipercept_amd", done
+
+
+def test_packaging_without_torch_leaves_out_its_operators_alone(tmp_path):
+    """A build environment of its own (pip's isolation) holds no torch: the C library is built as ever."""
+    block = tmp_path / "block"
+    block.mkdir()
+    (block / "torch.py").write_text("raise ModuleNotFoundError(\"No module named 'torch'\", name='torch')\n")
+    package, done = _packaging(tmp_path, PYTHONPATH=str(block))
+    assert done.returncode == 0, done.stderr
+    assert (package / "libmsda.so").exists() and not (package / "libmsda_torch.so").exists()
+    assert "--no-build-isolation" in done.stderr
+
+
+def test_packaging_compiles_the_torch_operators_for_the_torch_at_hand(tmp_path):
+    """Whatever is there may be another torch's: file times do not tell."""
+    package, done = _packaging(tmp_path)
+    assert done.returncode == 0, done.stderr
+    first = (package / "libmsda_torch.so").read_text(), (package / "libmsda.so").read_text()
+    package, done = _packaging(tmp_path)
+    assert done.returncode == 0, done.stderr
+    assert first == ("built\n", "built\n")
+    assert (package / "libmsda_torch.so").read_text() == "built\nbuilt\n"
+    assert (package / "libmsda.so").read_text() == "built\n"
+
+
 # ---- argument errors of the C ABI -------------------------------------------------------------------
 
 

@@ -169,7 +169,8 @@ def torch_ops():
                 if not TORCH_LIB_PATH.exists():
                     raise MsdaLibraryError(
                         f"{TORCH_LIB_PATH} not found: build it with `python -c 'import __graft_entry__ "
-                        "as g; g.build()'`. There is no fallback."
+                        "as g; g.build()'`, or install with `pip install --no-build-isolation .` (it is "
+                        "compiled against the installed torch). There is no fallback."
                     )
                 # the operators take the C entry points from the library that is loaded already
                 ctypes.CDLL(str(LIB_PATH), mode=ctypes.RTLD_GLOBAL)
