@@ -476,6 +476,50 @@ def test_group_norm_relu_gate_is_one_in_every_pass(case, dtype):
         check((name, case, dtype), t.grad, want, bound + half_step(want, t.grad.dtype))
 
 
+@pytest.mark.parametrize("dtype,c,groups", [(F32, 1024, 32), (F32, 1023, 33), (BF16, 2048, 64), (BF16, 2047, 23), (F64, 512, 16)])
+def test_group_norm_statistics_with_outliers(dtype, c, groups):
+    """170 rows a thread, which the small levels of the other tests never give, with values far from the
+    rest at the first rows of threads and in between.  A step of four rows adds five terms to a thread's
+    M2, none larger than M2 after it; lanes, chunks and groups join in fewer than 100 additions more."""
+    n, rows = 2, 170 * 1024
+    depth = 5 * (170 // 4 + 3) + 100
+    g = torch.Generator(device="cuda").manual_seed(3)
+    clean = torch.empty(n, rows, c, dtype=dtype, device="cuda").normal_(generator=g)
+    w = torch.ones(c, dtype=F64 if dtype == F64 else F32, device="cuda")
+    for far in (1e4, -3e6):
+        x = clean.clone()
+        x[0, 0] = x[1, 172 * 9] = x[1, 172 * 700 + 3] = x[1, 172 * 700 + 77] = far
+        _, mean, rstd = _lib.torch_ops().level_group_norm_fwd(x, w, w, groups, [rows], 1e-5, "none", True)
+        for i in range(n):
+            wide = x[i].double().view(rows, groups, c // groups)
+            exact_mean = wide.mean((0, 2))
+            exact = ((wide - exact_mean[:, None]).square().mean((0, 2)) + 1e-5).rsqrt()
+            size = wide.abs().mean((0, 2))
+            # (chunks of 172 rows join about the mean of the first, which an outlying row moves by far / 172)
+            check(("mean", i, far), mean[i, 0], exact_mean.cpu(), (depth * unit(dtype) * (size + abs(far) / 172)).cpu())
+            # half of the variance's relative error, two roundings of the root and the quotient
+            check(("rstd", i, far), rstd[i, 0], exact.cpu(), ((depth / 2 + 4) * unit(dtype) * exact).cpu())
+
+
+@pytest.mark.parametrize("c,groups", [(32, 4), (21, 3)])
+def test_group_norm_not_finite_groups_of_long_levels(c, groups):
+    """NaN and infinities stay in their (sample, level, group); a group without spread gives the bias."""
+    rows, per = [96 * 130, 5000], c // groups
+    x = normal((2, sum(rows), c), F32, 4).cuda()
+    one, zero = torch.ones(c, device="cuda"), torch.zeros(c, device="cuda")
+    shapes = [(96, 130), (50, 100)]
+    clean = level_group_norm(x, one, zero, groups, shapes)
+    for at, value in ((0, float("nan")), (rows[0] + 4321, float("inf")), (rows[0] - 1, float("-inf"))):
+        bad = x.clone()
+        bad[1, at, per + 1] = value
+        got = level_group_norm(bad, one, zero, groups, shapes)
+        hit = torch.zeros_like(got, dtype=torch.bool)
+        hit[1, (slice(0, rows[0]) if at < rows[0] else slice(rows[0], None)), per : 2 * per] = True
+        assert got[hit].isnan().all() and torch.equal(got[~hit], clean[~hit]), (at, value)
+    const = level_group_norm(torch.full_like(x, 7.0), one, zero + 0.25, groups, shapes)
+    assert torch.equal(const, torch.full_like(const, 0.25))
+
+
 def test_group_norm_empty_and_partial_gradients():
     w, b = torch.ones(8, device="cuda", requires_grad=True), torch.zeros(8, device="cuda", requires_grad=True)
     for shape in ((0, 5, 8), (3, 0, 8)):

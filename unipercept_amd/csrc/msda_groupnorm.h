@@ -59,24 +59,32 @@ __device__ __forceinline__ int gn_lane_rows(int rows, int r, int lanes) {
   return r < rows ? (rows - r + lanes - 1) / lanes : 0;
 }
 
-// Calls load(p, r) and use(p, r) for the thread's rows r0, r0 + lanes, ... of a chunk, the loads of
-// kGnRowsAhead rows issued before the first is used.
+// Walks the thread's rows r0, r0 + lanes, ... of a chunk in steps of kGnRowsAhead rows, and of one row
+// for the rest: load(p, r) for every row of a step, then use(p, r) with the array of the step's rows.
 template <typename P, typename Load, typename Use>
-__device__ __forceinline__ void gn_rows(int r0, int rows, int lanes, Load load, Use use) {
+__device__ __forceinline__ void gn_row_steps(int r0, int rows, int lanes, Load load, Use use) {
   constexpr int U = kGnRowsAhead;
   int r = r0;
   for (; r + (U - 1) * lanes < rows; r += U * lanes) {
     P p[U];
 #pragma unroll
     for (int k = 0; k < U; ++k) load(p[k], r + k * lanes);
-#pragma unroll
-    for (int k = 0; k < U; ++k) use(p[k], r + k * lanes);
-  }
-  for (; r < rows; r += lanes) {
-    P p;
-    load(p, r);
     use(p, r);
   }
+  for (; r < rows; r += lanes) {
+    P p[1];
+    load(p[0], r);
+    use(p, r);
+  }
+}
+// the same with use(p, r) for one row at a time
+template <typename P, typename Load, typename Use>
+__device__ __forceinline__ void gn_rows(int r0, int rows, int lanes, Load load, Use use) {
+  gn_row_steps<P>(r0, rows, lanes, load, [&](auto& p, int r) {
+    constexpr int K = sizeof(p) / sizeof(P);
+#pragma unroll
+    for (int k = 0; k < K; ++k) use(p[k], r + k * lanes);
+  });
 }
 
 // sums of two values over the `width` lanes of a team (a power of two up to the wave)
@@ -166,6 +174,10 @@ __device__ __forceinline__ CT gn_slope(CT z) {
   return CT(1);
 }
 
+// 1 / n of a count of rows, n >= 1 (v_rcp_f32 is within one step of it)
+__device__ __forceinline__ float gn_inverse(float n) { return __builtin_amdgcn_rcpf(n); }
+__device__ __forceinline__ double gn_inverse(double n) { return 1.0 / n; }
+
 // ---- the normalised value ---------------------------------------------------------------------------
 // z = (x - mean) * (rstd * weight) + bias decides the ReLU's gate, and an element whose z is a rounding
 // away from 0 has to be open in all of y, dx, dw and db or in none.  So every pass of both directions
@@ -187,9 +199,13 @@ __device__ __forceinline__ float gn_rstd(float sum, float inv, float eps) { retu
 
 // ---- forward ----------------------------------------------------------------------------------------
 // partial[(block * G + g) * 2] = (mean, M2) of the chunk's rows of group g.
-// Thread-level sums are taken about the first value that the thread reads of each channel, so a
-// common offset of the values costs nothing; an outlying first value costs at most a rounding per
-// row of what it adds to the variance itself.
+// A thread keeps the mean and M2 of the rows that it has read, per channel, and merges the next step's
+// k rows about that mean: with d_i = x_i - mean, D = sum d_i and n rows so far,
+//   mean += D / (n + k),  M2 += sum d_i^2 - D^2 / (n + k)
+// (k = 1 is Welford's recurrence).  D^2 / (n + k) takes away at most half of sum d_i^2, in the first step
+// (about its first row) three quarters, so nothing cancels: a common offset of the values costs nothing,
+// and an outlying value costs roundings of its own share of M2.  (Sums about the first value alone lose
+// about n^2 / 2 roundings where that value is the outlier.)
 // Where a vector lies in one group, a thread joins its VE channels before the workgroup does (10752 bf16
 // rows of 256 channels 6.6 -> 5.3 us, 348160 rows 33.3 -> 31.5).
 // Dynamic LDS: 2 * row lanes * C values.
@@ -211,51 +227,58 @@ __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(
   const int joined = whole ? VE : 1;  // channels of a part in LDS
   for (int k = threadIdx.x - r0 * vecs; k < vecs && r0 < lanes; k += kGnThreads) {
     const auto sp = Span<VE, MODE>::at(k, C);
-    // about the first row; a step has kGnRowsAhead rows in flight, the first row among them
-    ct pivot[VE], s[VE], q[VE];
+    ct mean[VE], m2[VE];
 #pragma unroll
-    for (int i = 0; i < VE; ++i) pivot[i] = s[i] = q[i] = 0;
-    bool first = true;
-    gn_rows<P>(
+    for (int i = 0; i < VE; ++i) mean[i] = m2[i] = 0;
+    int n = 0;
+    gn_row_steps<P>(
         r0, ch.rows, lanes, [&](P& p, int r) { sp.load(p, src + static_cast<int64_t>(r) * C); },
-        [&](P& p, int) {
-          ct v[VE];
-          p.unpack(v);
+        [&](auto& p, int) {
+          constexpr int K = sizeof(p) / sizeof(P);
+          ct v[K][VE];
+#pragma unroll
+          for (int k = 0; k < K; ++k) p[k].unpack(v[k]);
+          if (n == 0) {  // (the first step is taken about its first row)
+#pragma unroll
+            for (int i = 0; i < VE; ++i) mean[i] = v[0][i];
+          }
+          n += K;
+          const ct inv = gn_inverse(static_cast<ct>(n));
 #pragma unroll
           for (int i = 0; i < VE; ++i) {
-            if (first) pivot[i] = v[i];
-            const ct d = v[i] - pivot[i];
-            s[i] += d;
-            q[i] += d * d;
+            ct sum = v[0][i] - mean[i];
+            m2[i] += sum * sum;
+#pragma unroll
+            for (int k = 1; k < K; ++k) {
+              const ct d = v[k][i] - mean[i];
+              sum += d;
+              m2[i] += d * d;
+            }
+            const ct move = sum * inv;
+            m2[i] -= sum * move;
+            mean[i] += move;
           }
-          first = false;
         });
-    const int n = gn_lane_rows(ch.rows, r0, lanes);
-    const ct inv = n > 0 ? ct(1) / static_cast<ct>(n) : ct(0);
 #pragma unroll
-    for (int i = 0; i < VE; ++i) {
-      const ct m2 = q[i] - s[i] * s[i] * inv;
-      s[i] = pivot[i] + s[i] * inv;
-      q[i] = m2 < ct(0) ? ct(0) : m2;  // (NaN stays)
-    }
+    for (int i = 0; i < VE; ++i) m2[i] = m2[i] < ct(0) ? ct(0) : m2[i];  // (NaN stays)
     if (whole) {
-      ct d = 0, m2 = 0;
+      ct d = 0, all = 0;
 #pragma unroll
-      for (int i = 1; i < VE; ++i) d += s[i] - s[0];
+      for (int i = 1; i < VE; ++i) d += mean[i] - mean[0];
       d *= ct(1) / VE;
 #pragma unroll
       for (int i = 0; i < VE; ++i) {
-        const ct e = s[i] - s[0] - d;
-        m2 += q[i] + static_cast<ct>(n) * e * e;
+        const ct e = mean[i] - mean[0] - d;
+        all += m2[i] + static_cast<ct>(n) * e * e;
       }
-      lds_mean[r0 * vecs + k] = s[0] + d;
-      lds_m2[r0 * vecs + k] = m2;
+      lds_mean[r0 * vecs + k] = mean[0] + d;
+      lds_m2[r0 * vecs + k] = all;
     } else {
 #pragma unroll
       for (int i = 0; i < VE; ++i)
         if (sp.owns(i)) {
-          lds_mean[r0 * C + sp.c + i] = s[i];
-          lds_m2[r0 * C + sp.c + i] = q[i];
+          lds_mean[r0 * C + sp.c + i] = mean[i];
+          lds_m2[r0 * C + sp.c + i] = m2[i];
         }
     }
   }
