@@ -941,6 +941,38 @@ def test_encoder_layer_under_autocast():
     _close(a, b, 3e-2)
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("stream", [F32, "same"])
+def test_encoder_layer_with_16_bit_parameters_under_autocast(dtype, stream, monkeypatch):
+    monkeypatch.setenv("MSDA_DETERMINISTIC", "1")  # the attention's gradients with the same bits every time
+    plain, fused = (layer.to(dtype) for layer in _layer_pair(0.0))
+    src, pos, ref_points, shapes, lsi, dy = _layer_inputs()
+    if stream == "same":
+        src, pos = src.to(dtype), pos.to(dtype)
+    inputs = (src, pos, ref_points, shapes, lsi, dy)
+    with torch.autocast("cuda", dtype):
+        a, b = _train(fused, *inputs), _train(plain, *inputs)
+    assert a[0].dtype == F32
+    # The same values as fp32 parameters: every product runs in 16 bits and every norm in fp32 either way,
+    # so the results agree to the bit but for the parameters' own rounding of their gradients.
+    lifted = _layer_pair(0.0)[1]
+    lifted.load_state_dict({k: v.float() for k, v in fused.state_dict().items()})
+    with torch.autocast("cuda", dtype):
+        c = _train(lifted, *inputs)
+    assert all(torch.equal(x, y.to(x.dtype)) for x, y in zip(a, c))
+    # Against the plain layer.  Both routes round the same tensors, and sums kept in fp32 may land a whole
+    # step (eps of the value) apart at each; the longest path, to the gradient of the sampling offsets'
+    # weight, has 14 of them (query, its projection, value, attention, output projection, linear1, linear2;
+    # the gradients of linear2's output, hidden tensor, linear1's input, attention branch, output
+    # projection's input, sampling points, weight).  The ReLU's input differs by up to 2.5 steps (the sum
+    # that the plain route rounds, linear1's input, its output), which moves a share of 2.5 * 2 * eps *
+    # (density 0.4 of a normal variable at 0) = 2 eps of the units over 0, where half of them are open:
+    # sqrt(2 eps / 0.5) of the gradient's norm.
+    eps = torch.finfo(dtype).eps
+    _close(a[:1], b[:1], 14 * eps)
+    _close(a, b, 14 * eps + 2 * eps**0.5)
+
+
 def test_projection_and_encoder_train_together():
     """Input projections, then a stack with dropout: repeatable under one seed, new masks otherwise."""
     torch.manual_seed(5)

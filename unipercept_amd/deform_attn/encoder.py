@@ -85,6 +85,13 @@ def encoder_reference_points(
     return ref[:, :, None, :] * valid_ratios[:, None, :, :]
 
 
+def _autocast_to_fp32(t: torch.Tensor) -> torch.Tensor:
+    """What autocast does to the inputs of a norm: 16 bits become fp32, so its result is fp32."""
+    if torch.is_autocast_enabled("cuda") and t.dtype in (torch.bfloat16, torch.float16):
+        return t.float()
+    return t
+
+
 def _dropout_probability(module: nn.Module) -> float:
     """What the fused route takes from a layer's dropout module: its p while the module itself trains."""
     if type(module) is nn.Dropout:
@@ -153,17 +160,18 @@ class MSDeformAttnEncoderLayer(nn.Module):
         p = _dropout_probability(self.dropout)
         if p > 0.0 and rng_state is None:
             rng_state = new_rng_state(src.device)
-        if torch.is_autocast_enabled("cuda") and src.dtype in (torch.bfloat16, torch.float16):
-            src = src.float()  # autocast keeps the normalised stream in fp32
+        src = _autocast_to_fp32(src)  # the normalised stream
         norm1, norm2 = self.norm1, self.norm2
         src = dropout_add_layer_norm(
-            attn, src, norm1.weight, norm1.bias, p, rng_state, rng_site, norm1.eps
+            attn, src, _autocast_to_fp32(norm1.weight), _autocast_to_fp32(norm1.bias), p, rng_state,
+            rng_site, norm1.eps,
         )
         hidden = token_linear(src, self.linear1.weight, self.linear1.bias)
         hidden = counter_dropout(hidden, p, rng_state, rng_site + 1, "relu")
         ffn = token_linear(hidden, self.linear2.weight, self.linear2.bias)
         return dropout_add_layer_norm(
-            ffn, src, norm2.weight, norm2.bias, p, rng_state, rng_site + 2, norm2.eps
+            ffn, src, _autocast_to_fp32(norm2.weight), _autocast_to_fp32(norm2.bias), p, rng_state,
+            rng_site + 2, norm2.eps,
         )
 
 
