@@ -580,3 +580,19 @@ def test_input_projection_checks():
         LevelInputProjection([16], 20, 8)
     with pytest.raises(ValueError, match="levels"):
         LevelInputProjection([16, 32], 16, 4)([torch.zeros(1, 16, 2, 3)])
+
+
+def test_input_projection_takes_the_weights_of_convolutions_and_norms():
+    """The conversion that the documentation gives, from a state dict of (Conv2d, GroupNorm) pairs."""
+    nn = torch.nn
+    pairs = nn.ModuleList(nn.Sequential(nn.Conv2d(c, 16, 1), nn.GroupNorm(4, 16)) for c in (8, 24))
+    sd, levels = pairs.state_dict(), 2
+    proj = LevelInputProjection([8, 24], 16, 4)
+    proj.load_state_dict({
+        **{f"projections.{l}.weight": sd[f"{l}.0.weight"].flatten(1) for l in range(levels)},
+        **{f"projections.{l}.bias": sd[f"{l}.0.bias"] for l in range(levels)},
+        "norm_weight": torch.stack([sd[f"{l}.1.weight"] for l in range(levels)]),
+        "norm_bias": torch.stack([sd[f"{l}.1.bias"] for l in range(levels)]),
+    })
+    assert torch.equal(proj.projections[1].weight, pairs[1][0].weight[:, :, 0, 0])
+    assert torch.equal(proj.norm_bias[1], pairs[1][1].bias)

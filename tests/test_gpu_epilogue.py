@@ -1006,6 +1006,35 @@ def test_projection_and_encoder_train_together():
                            enc(src, shapes, lsi, pos=pos, spatial_shapes_list=levels))
 
 
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_projection_under_autocast(dtype):
+    """As a convolution and torch's group norm under autocast: 16-bit products, the norm's result and the
+    position embeddings in fp32."""
+    torch.manual_seed(7)
+    proj = LevelInputProjection([24, 40], 64, 16, "relu").cuda()
+    maps = [normal((2, 24, 8, 12), F32, 1).cuda(), normal((2, 40, 4, 6), F32, 2).cuda()]
+    with torch.autocast("cuda", dtype):
+        got, _, _, _, pos = proj(maps, position_feats=32)
+        want = flatten_levels([
+            torch.relu(torch.nn.functional.group_norm(
+                torch.nn.functional.conv2d(m, p.weight[:, :, None, None], p.bias), 16,
+                proj.norm_weight[i], proj.norm_bias[i]))
+            for i, (m, p) in enumerate(zip(maps, proj.projections))])[0]
+    assert got.dtype == want.dtype == pos.dtype == F32
+    assert (got - want).norm() <= 3 * torch.finfo(dtype).eps * want.norm()
+    # the norm's result is not rounded to 16 bits: most values lie between two of them
+    assert (got.to(dtype).float() != got)[got > 0].double().mean() > 0.9
+    (grad,) = torch.autograd.grad(got.square().sum(), proj.norm_weight)
+    assert grad.dtype == F32 and torch.isfinite(grad).all()
+    # 16-bit parameters: the bits of the same values in fp32
+    proj.to(dtype)
+    wide = LevelInputProjection([24, 40], 64, 16, "relu").cuda()
+    wide.load_state_dict({k: v.float() for k, v in proj.state_dict().items()})
+    with torch.autocast("cuda", dtype):
+        assert torch.equal(proj(maps)[0], wide(maps)[0])
+    assert torch.equal(pos, flatten_levels([m[:, :24] for m in maps], 32)[4])
+
+
 def test_projection_gradients_match_convolutions():
     """Many tokens (the projections' weight gradients by slices), channels-last and plain maps:
     outputs and gradients against 1 x 1 convolutions and torch's group norm in fp64."""

@@ -243,7 +243,12 @@ class LevelInputProjection(nn.Module):
     ``forward(features)`` takes the (N, C_l, H_l, W_l) maps and returns what ``flatten_levels``
     returns for the projected maps.  The convolutions run as token GEMMs on the channels-last maps,
     the norms of all levels as one ``level_group_norm`` over the flattened pyramid (parameters
-    ``norm_weight`` and ``norm_bias`` (L, d_model), one set a level); ROCm tensors only."""
+    ``norm_weight`` and ``norm_bias`` (L, d_model), one set a level); ROCm tensors only.  Under autocast
+    the norms and what they return are fp32, as torch's group norm is.
+
+    A state dict of per-level ``(nn.Conv2d(c, d_model, 1), nn.GroupNorm)`` pairs does not load as it is:
+    ``projections.l.weight`` is the convolution's weight with its two spatial dimensions taken off,
+    ``projections.l.bias`` its bias, and ``norm_weight[l]``, ``norm_bias[l]`` are the norm's."""
 
     def __init__(
         self,
@@ -272,9 +277,11 @@ class LevelInputProjection(nn.Module):
         maps = []
         for f, proj in zip(features, self.projections):
             tokens = token_linear(f.permute(0, 2, 3, 1), proj.weight, proj.bias)
+            tokens = _autocast_to_fp32(tokens)  # before the flattening: the embeddings take its type
             maps.append(tokens.permute(0, 3, 1, 2))  # a view, as flatten_levels takes it
         src, spatial_shapes, level_start_index, shapes, pos = flatten_levels(maps, position_feats)
         src = level_group_norm(
-            src, self.norm_weight, self.norm_bias, self.num_groups, shapes, self.eps, self.activation
+            src, _autocast_to_fp32(self.norm_weight), _autocast_to_fp32(self.norm_bias), self.num_groups,
+            shapes, self.eps, self.activation,
         )
         return src, spatial_shapes, level_start_index, shapes, pos
