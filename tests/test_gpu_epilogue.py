@@ -757,6 +757,56 @@ def test_gradients_beyond_32_bit_offsets():
     assert ((gx[-1:].float() - last[0].float()).abs() <= 2.0**-7 * last[0].float().abs() + 1e-6).all()
 
 
+def test_parameter_gradients_beyond_32_bit_offsets():
+    """Sums over more than 2^31 elements against sums of blocks in fp64, from the forward's statistics.
+    A workgroup adds up to 256 rows a thread and the rest is joined by lanes: fewer than 400 additions deep."""
+    n, s, c, groups = 4, 1 << 17, 4112, 16
+    g = torch.Generator(device="cuda").manual_seed(2)
+    x = torch.empty(n, s, c, dtype=BF16, device="cuda").normal_(generator=g)
+    dy = torch.empty(n, s, c, dtype=BF16, device="cuda").normal_(generator=g)
+    assert x.numel() > 2**31
+    w = torch.ones(c, device="cuda").normal_(1.0, 0.3, generator=g)
+    b = torch.zeros(c, device="cuda").normal_(0.0, 0.3, generator=g)
+    op, r, depth = _lib.torch_ops(), 2.0**-24, 400
+
+    def compare(name, got, terms):
+        """terms(i, rows) -> the summands of (dw, db) for rows of sample i, and the error of a summand."""
+        sums = [torch.zeros(c, dtype=F64, device="cuda") for _ in range(4)]
+        for i in range(n):
+            for at in range(0, s, 1 << 13):
+                a, d, ea, ed = terms(i, slice(at, at + (1 << 13)))
+                for total, part in zip(sums, (a, d, depth * r * a.abs() + ea, depth * r * d.abs() + ed)):
+                    total += part.sum(0)
+        for k, what in enumerate(("dw", "db")):
+            check((name, what), got[k], sums[k].cpu(), sums[2 + k].cpu() + half_step(sums[k].cpu(), F32))
+
+    _, mean, rstd = op.level_group_norm_fwd(x, w, b, groups, [], 1e-5, "silu", True)
+    _, gw, gb = op.level_group_norm_bwd(dy, x, w, b, mean, rstd, groups, [], "silu", False, True)
+
+    def group_terms(i, rows):
+        mu, s_ = (t[i, 0].double().repeat_interleave(c // groups) for t in (mean, rstd))
+        u, d = (x[i, rows].double() - mu) * s_, dy[i, rows].double()
+        z = u * w.double() + b.double()
+        sig = torch.sigmoid(z)
+        dz = d * sig * (1 + z * (1 - sig))
+        # the slope: its own roundings, and those of z (|slope'| <= 0.5)
+        e = d.abs() * r * ((2 * z.abs() + 8) * (z.abs() + 1) + 0.5 * 5 * (u * w).abs() + 2 * b.abs()) + 2 * r * dz.abs()
+        return dz * u, dz, e * u.abs() + 4 * r * (dz * u).abs(), e
+
+    compare("group norm", (gw, gb), group_terms)
+    flat = x.view(-1, c)
+    _, mean, rstd = op.dropout_add_norm_fwd(flat, flat, w, b, None, 0.0, 0, 1e-5, True)
+    _, _, gw, gb = op.dropout_add_norm_bwd(dy.view(-1, c), flat, flat, w, mean, rstd, None, 0.0, 0, False, False, True)
+
+    def norm_terms(i, rows):
+        at = slice(i * s + rows.start, i * s + rows.stop)
+        u = (2 * flat[at].double() - mean[at, None].double()) * rstd[at, None].double()
+        d = dy[i, rows].double()
+        return d * u, d, 4 * r * (d * u).abs(), 0 * d
+
+    compare("residual norm", (gw, gb), norm_terms)
+
+
 @pytest.mark.parametrize("dtype,c,groups", [(BF16, 8192, 1), (F16, 8191, 1), (F32, 4096, 1), (F32, 4095, 3), (F64, 2047, 1),
                                             (BF16, 8192, 8192), (F32, 4096, 32)])
 def test_group_norm_widest_rows(dtype, c, groups):
