@@ -97,6 +97,28 @@ def test_oracle_gradients_against_differences(activation):
             assert abs(got - (grads[k] * d).sum().item()) < 1e-6 * (1 + abs(got))
 
 
+def test_normal_distribution_fit():
+    """The constants of gn_phi, as fp32 holds them, against the complementary error function: the error
+    that the kernel's comment states, without the kernel's own roundings."""
+    import re
+    from pathlib import Path
+
+    from scipy.special import erfc
+
+    source = (Path(_lib.__file__).parent / "csrc" / "msda_groupnorm.h").read_text()
+    body = source[source.index("float gn_phi(float z, float& e)") :]
+    body = body[: body.index("\n}")]
+    step = float(np.float32(re.search(r"1\.f \+ ([0-9.]+)f \* a", body).group(1)))
+    first = re.search(r"float r = (-?[0-9.]+)f;", body).group(1)
+    rest = re.findall(r"r = r \* t ([+-]) ([0-9.]+)f;", body)
+    coefficients = [float(np.float32(v)) for v in (first, *(sign + value for sign, value in rest))]
+    assert len(coefficients) == 7
+    a = np.linspace(0.0, 8.0, 400001)
+    t = 1 / (1 + step * a)
+    upper = np.polyval([*coefficients, 0.0], t) * np.exp(-0.5 * a * a)
+    assert np.abs(upper - 0.5 * erfc(a * 0.5**0.5)).max() <= 8.4e-9
+
+
 # ---- refusals of the Python surface -----------------------------------------------------------------
 
 

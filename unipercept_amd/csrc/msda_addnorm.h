@@ -16,7 +16,7 @@
 // h and all sums are in 32 bits (64 for fp64).
 //
 // Bound by HBM where rows are many (MI355X, 344064 rows of 256 fp32 columns, dropout 0.1): forward
-// 1.06 GB in 168 us, 6.3 TB/s; backward 1.78 GB in 290 us, 6.1 TB/s, and 15 us for the column sums.
+// 1.06 GB in 168 us, 6.3 TB/s; backward 1.78 GB in 293 us, 6.1 TB/s, and 15 us for the column sums.
 #pragma once
 
 #include "msda_dropout.h"

@@ -72,7 +72,7 @@ __device__ __forceinline__ uint32_t keep_bits(const DropKey& key, uint64_t first
 // compute it, which leaves the arithmetic per byte that of the 16-bit types (two vectors a lane
 // instead leave every access half a line: 54 MB in 44 us against 20).  RELU: y = max(x, 0) first
 // (NaN stays); a dropped element is 0 whatever x holds.
-// Bound by HBM: 344064 x 1024 bf16 with ReLU and dropout, 1.41 GB in 225 us, 6.2 TB/s; the generator
+// Bound by HBM: 344064 x 1024 bf16 with ReLU and dropout, 1.41 GB in 234 us, 6.0 TB/s; the generator
 // fills 0.6 of the VALU's time beside it (86 M wave instructions).
 template <typename T, bool RELU, bool DROP>
 __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T* __restrict__ out,
@@ -113,7 +113,7 @@ __global__ __launch_bounds__(256) void dropout_kernel(const T* __restrict__ x, T
 
 // Gradient of ReLU + dropout from the stored output: y is 0 exactly where the element was dropped
 // or the ReLU closed (x * scale cannot underflow, scale >= 1), so the mask needs no generator.
-// Bound by HBM: the same tensors, 2.11 GB in 322 us, 6.5 TB/s.
+// Bound by HBM: the same tensors, 2.11 GB in 323 us, 6.5 TB/s.
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_relu_bwd_kernel(
     const T* __restrict__ grad_out, const T* __restrict__ y, T* __restrict__ grad_x, int64_t numel,

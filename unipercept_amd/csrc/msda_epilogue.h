@@ -31,8 +31,9 @@ inline bool drop_args(double p, DropArgs* a) {
 constexpr int64_t kMaxDropElements = static_cast<int64_t>(1) << 35;  // 32-bit block counter
 
 // Workgroups of a pass over `items` steps of `per_block` a workgroup: one step each, so that loads
-// of the next workgroups overlap the stores of the last (a copy of 352 MB runs at 6.7 TB/s so and
-// at 5.8 with 2048 workgroups that loop); more than a launch holds are looped over.
+// of the next workgroups overlap the stores of the last (a copy of 352 MB, one vector a thread and
+// step: 6.8 TB/s so with the streaming hint and 6.1 without, 5.7 and 5.0 with 2048 workgroups that
+// loop); more than a launch holds are looped over.
 inline unsigned pass_grid(int64_t items, int per_block) {
   const int64_t blocks = (items + per_block - 1) / per_block;
   return static_cast<unsigned>(blocks < (1 << 23) ? blocks : (1 << 23));
@@ -99,7 +100,10 @@ inline int add_norm_check(int64_t rows, int C, double p, int site, int dtype_x, 
 // (the backward keeps more of a row in registers and gains less from the shorter sums).
 // Rows between two shapes take one that leaves few lanes empty (fp16, forward, 21502 rows of 520
 // columns, 65 vectors: 64 x 2 19.0, 32 x 3 15.9; of 1030, 129 vectors: 64 x 4 48, 64 x 3 34; of 258,
-// 33 vectors: 64 x 1 15.5, 16 x 3 11.0).
+// 33 vectors: 64 x 1 15.5, 16 x 3 11.0).  16 x 3, 32 x 3, 64 x 3 and 64 x 4 were chosen by these times of
+// the forward and serve the backward too, where no other shape was timed (fp16, 21502 rows with the column
+// sums: 16 x 3, 258 columns 38 us; 32 x 3, 515 columns 50; 64 x 3, 1030 columns 75; 64 x 4, 1537 columns
+// 153 where 1536 take 77: on odd 16-bit rows that one uses all 256 registers and spills about 20).
 struct AddNormTeam {
   int TS, NV;
 };

@@ -13,8 +13,8 @@
 // thread, all their loads in flight at once), which need the level's joined sums and not its chunks'.
 //
 // Bound by HBM, which every tensor but the last crosses twice a direction (MI355X, 8 x 43008 rows of
-// 256 fp32 channels, 352 MB a tensor): sums 56 us, 6.3 TB/s; forward pass 112 us, 6.3 TB/s; sums of
-// the gradient 113 us, 6.2 TB/s; its pass 162 us, 6.5 TB/s; the joins 5 and 6 us.
+// 256 fp32 channels, 352 MB a tensor): sums 56 us, 6.3 TB/s; forward pass 113 us, 6.2 TB/s; sums of
+// the gradient 115 us, 6.1 TB/s; its pass 162 us, 6.5 TB/s; the joins 5 and 6 us.
 #pragma once
 
 #include "msda_vec.h"
@@ -125,9 +125,10 @@ __device__ __forceinline__ double gn_sigmoid(double z) { return 1.0 / (1.0 + exp
 
 // Normal distribution function Phi(z) and, with it, exp(-z^2 / 2).  In fp32
 //   1 - Phi(a) = exp(-a^2 / 2) * R(t),  t = 1 / (1 + 0.46 a),  a = |z|,
-// with a polynomial R of degree 7 without constant term, fitted to sqrt(2 pi)^-1 times Mills' ratio for
-// the least maximum error of the product over a = 0 .. 8: 4.5e-9, a tenth of fp32's rounding of Phi.
-// (Parameters' gradients add this error up with one sign: a form that is off by 1.5e-7 shows there.)
+// with a polynomial R of degree 7 without constant term, fitted to sqrt(2 pi)^-1 times Mills' ratio over
+// a = 0 .. 8.  With these constants as fp32 holds them the product is off by at most 8.4e-9 (at a = 0.74),
+// 0.28 of fp32's rounding of a Phi next to 1.  (Parameters' gradients add this error up with one sign: a
+// form that is off by 1.5e-7 shows there.)
 // One exponential serves the function and its density.
 __device__ __forceinline__ float gn_phi(float z, float& e) {
   const float a = fabsf(z);
@@ -207,7 +208,7 @@ __device__ __forceinline__ float gn_rstd(float sum, float inv, float eps) { retu
 // and an outlying value costs roundings of its own share of M2.  (Sums about the first value alone lose
 // about n^2 / 2 roundings where that value is the outlier.)
 // Where a vector lies in one group, a thread joins its VE channels before the workgroup does (10752 bf16
-// rows of 256 channels 6.6 -> 5.3 us, 348160 rows 33.3 -> 31.5).
+// rows of 256 channels 5.4 us, 348160 rows 32.3; 1.3 and 1.8 us more where the workgroup joins them).
 // Dynamic LDS: 2 * row lanes * C values.
 template <typename T, int MODE>
 __global__ __launch_bounds__(kGnThreads) void gn_stats_kernel(
