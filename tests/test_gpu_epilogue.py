@@ -890,6 +890,22 @@ def test_function_transforms_are_right_or_refused():
         assert torch.equal(got, want)
 
 
+def test_vmap_draws_the_masks_of_its_states():
+    x = normal((3, 10, 24), F32, 1).cuda().requires_grad_(True)
+    states = torch.stack([rng((k, 7 - k)) for k in range(3)])
+    w, b = normal((24,), F32, 2).cuda(), normal((24,), F32, 3).cuda()
+    dy = normal((3, 10, 24), F32, 4).cuda()
+    for f in (lambda t, state: counter_dropout(t, 0.4, state, 1, "relu"),
+              lambda t, state: dropout_add_layer_norm(t, t, w, b, 0.4, state, 2)):
+        for mode, in_dims, state in (("different", (0, 0), states), ("error", (0, 0), states), ("same", (0, None), states[0])):
+            got = torch.func.vmap(f, in_dims=in_dims, randomness=mode)(x, state)
+            want = torch.stack([f(x[k], state if in_dims[1] is None else state[k]) for k in range(3)])
+            assert torch.equal(got, want)
+            assert torch.equal(*(torch.autograd.grad(t, x, dy)[0] for t in (got, want)))
+        with pytest.raises(RuntimeError, match="same mask"):
+            torch.func.vmap(lambda t: f(t, states[0]), randomness="different")(x)
+
+
 def test_two_threads_at_once():
     """Calls of two host threads on streams of their own."""
     import threading
